@@ -66,9 +66,10 @@ def draw(rng):
         h, w = _log_int(rng, 1, 128), _log_int(rng, 1, 128)
         if h * w * (channels // groups) < 16:                      # fewer values have a gradient that is all cancellation
             w = 16
-        b = _log_int(rng, 1, max(1, min(48, (1 << 25) // (channels * h * w))))
+        t = rng.choice(["bf16", "bf16", "f32"])
+        b = _log_int(rng, 1, max(1, min(48, (1 << (25 if t == "bf16" else 24)) // (channels * h * w))))
         c = _gn("", batch=b, height=h, width=w, channels=channels, groups=groups, act=rng.choice(["none", "silu", "lrelu"]),
-                dtype=rng.choice(["bf16", "bf16", "f32"]), train=rng.random() < 0.6)
+                dtype=t, train=rng.random() < 0.6)
     else:
         train = rng.random() < 0.6
         d, kv, rep = rng.choice([32, 64, 128]), rng.choice([1, 1, 2, 4]), rng.choice([1, 1, 2, 3])
