@@ -26,7 +26,7 @@
 extern "C" {
 #endif
 
-#define RGBD_ABI_VERSION 20
+#define RGBD_ABI_VERSION 21
 
 int rgbd_abi_version(void);
 const char* rgbd_last_error(void);
@@ -582,6 +582,59 @@ int rgbd_adam_clip_multi(float* p, float* g, float* m, float* v, int64_t n,
                          int nseg, const int64_t* seg_begin, const float* seg_alpha,
                          float beta1, float beta2, float eps, float clip, float grad_scale,
                          int32_t* step, float* workspace, float* norm_out, void* stream);
+
+/* ------------------------------------------------------------------ group normalisation, channels last
+ * x (B, N, C), C channels in `groups` groups of neighbours; per sample and group the mean and variance over its N * C / groups
+ * values (biased, like the instance norm above), y = act((x - mean) * rstd * gamma[c] + beta[c]).
+ *   dtype 0: x, y, dy, dx bf16; 1: fp32.  gamma, beta, dgamma, dbeta, mean, rstd fp32; mean, rstd (B, groups).
+ *   act 0: none; 1: leaky ReLU (slope for z <= 0); 2: SiLU z / (1 + exp(-z)).
+ *   workspace: rgbd_group_norm_workspace floats, uninitialised.  Sums are ordered by the shape alone (no atomics).
+ *   C: at most 8192 (bf16) / 4096 (fp32); 1024 where C is no multiple of a 16-byte vector or a buffer is not 16-byte aligned.
+ * _bwd writes (does not accumulate) dx, dgamma, dbeta; B or N 0: dgamma, dbeta = 0. */
+int64_t rgbd_group_norm_workspace(int B, int N, int C, int groups, int dtype, int backward);   /* floats; -1: bad sizes */
+int rgbd_group_norm_fwd(const void* x, const float* gamma, const float* beta, void* y, float* mean, float* rstd,
+                        float* workspace, int B, int N, int C, int groups, int dtype, int act, float eps, float slope, void* stream);
+int rgbd_group_norm_bwd(const void* x, const void* dy, const float* gamma, const float* beta, const float* mean, const float* rstd,
+                        void* dx, float* dgamma, float* dbeta, float* workspace, int B, int N, int C, int groups, int dtype, int act,
+                        float slope, void* stream);
+
+/* ------------------------------------------------------------------ attention over the tokens of a pixel grid
+ * q (B, Lq, H, D), k, v (B, Lk, Hkv, D) bf16 at any strides (elements, multiples of 8; the D values of a head are contiguous, the
+ * pointers 16-byte aligned), D in {32, 64, 128}, Hkv divides H: head h reads key / value head h / (H / Hkv).
+ *   s = scale q.k;  cap > 0: s = cap tanh(s / cap);  table: s += table[h][map[offset]];  keys j >= lengths[b] are left out
+ *   (lengths NULL: none; values are clamped to [0, Lk]);  o = softmax(s) v, 0 where a row has no key.
+ * With a table, query i is token q_start + i and key j token j of a rows x cols grid in raster order, and the offset of a pair is
+ *   (row_i - row_j + rows - 1) * (2 cols - 1) + (col_i - col_j + cols - 1);  map (2 rows - 1)(2 cols - 1) int32 bucket numbers
+ *   (clamped to [0, n_buckets)), table (H, n_buckets) fp32.  rows == 1, or cols <= 1024.
+ * o, o_lo (B, Lq, H, D) contiguous bf16: the output and (may be NULL) what rounding it dropped; lse (B, H, Lq) fp32 (may be NULL):
+ *   log2 of the row's sum of exp, in units of log2 -- o_lo and lse are what the backward pass needs.  fine != 0: the probabilities
+ *   enter the second product with 16 bits instead of 8, which the table's gradient needs to be exact to fp32's last digits. */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+    const float* table;
+    const int32_t* map;
+    const int32_t* lengths;
+    float* lse;
+    int B, H, Hkv, Lq, Lk, D;
+    int rows, cols, q_start, n_buckets;
+    float scale, cap;
+    int fine;
+} rgbd_attn_desc;
+/* d_o, o, o_lo (B, Lq, H, D) contiguous; dq, dk, dv bf16 at any strides (multiples of 8); dtable (H, n_buckets) fp32 or NULL.
+ * order / start: the offsets of each bucket, bucket u's are order[start[u]] .. order[start[u + 1] - 1].  Gradients are written, not
+ * accumulated, for every row (0 for keys at or beyond the length), and every sum has one order: results repeat bit for bit. */
+typedef struct {
+    const void *d_o, *o, *o_lo;
+    void *dq, *dk, *dv;
+    int64_t dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
+    float* dtable;
+    const int32_t* order;
+    const int32_t* start;
+} rgbd_attn_grad;
+int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, void* stream);
+int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table);                 /* floats; -1: bad sizes */
+int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream);
 
 #ifdef __cplusplus
 }

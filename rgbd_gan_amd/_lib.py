@@ -10,7 +10,7 @@ from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_void_p, POINTER
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # RGBD_LIB_PATH: A/B timing of another build of the same ABI; the default is the in-tree library
 LIB_PATH = os.environ.get("RGBD_LIB_PATH") or os.path.join(_HERE, "librgbdgan_hip.so")
-ABI_VERSION = 20
+ABI_VERSION = 21
 
 _P = c_void_p
 
@@ -123,6 +123,12 @@ PROTOTYPES = {
     "rgbd_nonfinite_mask_f32": ([POINTER(c_void_p), c_int, _P, _P], c_int),
     "rgbd_adam_clip_multi": ([_P, _P, _P, _P, c_int64, c_int, POINTER(c_int64), POINTER(c_float), c_float, c_float,
                               c_float, c_float, c_float, _P, _P, _P, _P], c_int),
+    "rgbd_group_norm_workspace": ([c_int, c_int, c_int, c_int, c_int, c_int], c_int64),
+    "rgbd_group_norm_fwd": ([_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, _P], c_int),
+    "rgbd_group_norm_bwd": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P], c_int),
+    "rgbd_attention_fwd": ([_P, _P, _P, _P], c_int),
+    "rgbd_attention_bwd_workspace": ([_P, c_int], c_int64),
+    "rgbd_attention_bwd": ([_P, _P, _P, _P], c_int),
 }
 
 _lib = None

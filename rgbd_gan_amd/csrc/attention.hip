@@ -1,0 +1,920 @@
+// Attention over the tokens of a pixel grid with a learned relative position bias, forward and backward.
+//
+//   s_ij = scale q_i . k_j;  cap > 0: s_ij = cap tanh(s_ij / cap);  s_ij += table[h][bucket(offset of i from j)];
+//   keys j >= lengths[b] do not exist;  p = softmax over the keys;  o_i = sum_j p_ij v_j, and 0 for a row without keys.
+//   ds = p (dp - delta), dp_ij = do_i . v_j, delta_i = do_i . o_i;  dtable[h][u] = sum of ds over the pairs of bucket u;
+//   through the cap ds (1 - tanh^2);  dq = scale ds k, dk = scale ds^T q, dv = p^T do.
+//
+// Token t sits at row t / cols, column t % cols of the grid.  With P(t) = t + (cols - 1) (t / cols) the offset (dy, dx) of a
+// pair is the single number P(i) - P(j), so the bias of a tile of scores is a short run of the (2 rows - 1)(2 cols - 1) offsets.
+//
+// Matrix products run on v_mfma_f32_32x32x16_bf16.  Scores are computed TRANSPOSED (keys x queries: the keys are the A
+// operand), so a lane holds one query and 16 of its keys: row maximum and sum need one exchange between lane l and l + 32,
+// the rescaling of the output is one factor a lane, and the 16 probabilities are, packed to bf16, the B operand of the second
+// product as they stand (its K order follows the accumulator's: 4 keys of one half, 4 of the other), while the A operand comes
+// out of LDS through the transposing read.  Probabilities and score gradients are rounded to bf16 only as operands of these
+// products; maxima, sums, statistics and the table's gradient stay in fp32.
+#include "common.h"
+
+namespace {
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int KT = 64;                    // rows of a streamed tile (keys forward and in dq, queries in dk / dv)
+constexpr int BLK = 128;                  // rows a workgroup owns: 4 waves x 32
+constexpr int WIN_FLOATS = 8192;          // LDS floats for a window of the bias (32 KB): it spans as many tiles as fit
+constexpr int WIN_PAD = 4;
+constexpr float NEG_INF = -__builtin_inff();
+
+struct AttnArgs {
+    const unsigned short *q, *k, *v, *d_o, *o, *o_lo;
+    unsigned short *out, *out_lo, *dq, *dk, *dv;
+    float *lse, *delta, *part, *dtable;
+    const float* table; const int* map; const int* lengths;
+    int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
+    int64_t dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
+    int B, H, Hkv, rep, Lq, Lk;
+    int rows, cols, q_start, n_buckets;
+    int n_qb, n_kb, seg_tiles;
+    int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
+    float scale, cap;
+};
+
+// ---- positions
+__device__ __forceinline__ int pos_of(int t, int cols) { return t + (cols - 1) * (t / cols); }
+
+// ---- LDS tiles: `rows` x D bf16, 16-byte chunks permuted so that both ways of reading a tile spread over the 64 banks: the
+//      row-major 16-byte reads of 32 consecutive rows and the transposing 8-byte reads of 4 consecutive rows x 64 bytes.
+template <int D> __device__ __forceinline__ int swz(int row) {
+    if (D == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+    if (D == 64) return (((row >> 1) & 1) << 2) | (((row >> 2) & 1) << 1) | ((row >> 3) & 1);
+    return (row >> 2) & 3;
+}
+
+template <int D> struct Frags {
+    int rb;                               // row-major fragment: byte address of (row lane & 31, chunk lane / 32)
+    int tb;                               // transposed fragment: (row 4 (lane / 32) + q, columns 16 mblk + 4 p)
+    __device__ __forceinline__ Frags(int lane) {
+        const int r = lane & 31, half = lane >> 5;
+        rb = r * (2 * D) + ((half ^ swz<D>(r)) << 4);
+        const int q = (lane & 15) >> 2, p = lane & 3, mblk = (lane >> 4) & 1;
+        const int row = 4 * half + q;
+        tb = row * (2 * D) + (((mblk * 2 + (p >> 1)) ^ swz<D>(row)) << 4) + (p & 1) * 8;
+    }
+    // rows row0 .. row0 + 31 (row0 a multiple of 32), columns 16 ks + 8 half + 0..7
+    __device__ __forceinline__ bf16x8 row(const char* tile, int row0, int ks) const {
+        return *reinterpret_cast<const bf16x8*>(tile + row0 * (2 * D) + (rb ^ (ks << 5)));
+    }
+    // column 32 dblk + (lane & 31) of rows row0 + {4 half + 0..3, 8 + 4 half + 0..3} (row0 a multiple of 16)
+    __device__ __forceinline__ bf16x8 col(const char* tile, int row0, int dblk) const {
+        constexpr int EX = D == 64 ? 16 : 32;        // what row + 8 changes in swz
+        const char* t = tile + row0 * (2 * D);
+        const s16x4 a = tr(t + (tb ^ (dblk << 6)));
+        const s16x4 b = tr(t + 16 * D + (tb ^ EX ^ (dblk << 6)));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+    static __device__ __forceinline__ s16x4 tr(const char* p) {
+        return __builtin_amdgcn_ds_read_tr16_b64_v4i16((s16x4 __attribute__((address_space(3)))*)(const_cast<char*>(p)));
+    }
+};
+
+// One tile of KT rows x D from global memory into LDS through registers; rows at or beyond `valid` become zeros (whatever the
+// memory holds there, a NaN included).
+template <int D> struct Stage {
+    static constexpr int CH = D / 8, NP = KT * CH / 256;
+    u32x4 r[NP];
+    __device__ __forceinline__ void load(const unsigned short* base, int64_t sl, int row0, int valid) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int pc = threadIdx.x + 256 * i, row = row0 + pc / CH, ch = pc % CH;
+            if (row < valid) r[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)row * sl + ch * 8);
+            else r[i] = u32x4{0, 0, 0, 0};
+        }
+    }
+    __device__ __forceinline__ void store(char* tile) const {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int pc = threadIdx.x + 256 * i, row = pc / CH, ch = pc % CH;
+            *reinterpret_cast<u32x4*>(tile + row * (2 * D) + ((ch ^ swz<D>(row)) << 4)) = r[i];
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ bf16x8 pack8(const f32x16& v, int i0) {
+    u32x4 o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(v[i0 + 2 * i], v[i0 + 2 * i + 1]);
+    return __builtin_bit_cast(bf16x8, o);
+}
+__device__ __forceinline__ float other_half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
+__device__ __forceinline__ float other_half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
+
+// tanh of 16 values.  Below 0.5 an odd polynomial (least squares on Chebyshev nodes, relative error 1.1e-7: there the quotient
+// form would lose digits by cancellation, and capped scores mostly lie there); beyond it 1 - 2 / (e^2x + 1).
+__device__ __forceinline__ float tanh_small(float x) {
+    const float u = x * x;
+    float r = 0.017141319811344147f;
+    r = r * u + -0.05298924073576927f;
+    r = r * u + 0.13324828445911407f;
+    r = r * u + -0.3333307206630707f;
+    r = r * u + 1.f;
+    return r * x;
+}
+__device__ __forceinline__ void tanh16(f32x16& v, float f) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) { v[i] *= f; top = fmaxf(top, fabsf(v[i])); }
+    if (!__any(top >= 0.5f)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = tanh_small(v[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float e = __builtin_amdgcn_exp2f(2.f * LOG2E * v[i]);
+            const float t = 1.f - 2.f * __builtin_amdgcn_rcpf(e + 1.f);
+            v[i] = fabsf(v[i]) < 0.5f ? tanh_small(v[i]) : t;
+        }
+    }
+}
+
+// The workgroup's place: consecutive ids go round the 8 XCDs, so give each XCD a run of neighbours (they share keys and values).
+__device__ __forceinline__ int xcd_run(int id, int total) {
+    const int q = total >> 3, r = total & 7, x = id & 7;
+    return x * q + min(x, r) + (id >> 3);
+}
+
+// ---- the bias of a run of tiles, in LDS.  `own` = the workgroup's rows (first P, last P), `other` = the streamed rows.  Entry j is
+//      the offset whose place grows with the streamed row, so a lane reads upwards; SIGN: +1 streamed rows are queries.
+//      Values are kept times log2(e): the softmax runs on exp2.
+template <int SIGN>
+__device__ __forceinline__ void stage_window(float* win, const AttnArgs& a, int h, int own_first, int own_last, int other_first,
+                                             int other_last) {
+    const int n = (own_last - own_first) + (other_last - other_first) + 1;
+    const int c0 = (2 * a.cols - 1) * (a.rows - 1) + a.cols - 1;
+    const float* row = a.table + (int64_t)h * a.n_buckets;
+    const int base = SIGN > 0 ? other_first - own_last + c0 : own_last - other_first + c0;
+    for (int j = threadIdx.x; j < n; j += 256) {
+        int u = a.map[base + SIGN * j];
+        u = min(max(u, 0), a.n_buckets - 1);
+        win[j] = row[u] * LOG2E;
+    }
+    if (threadIdx.x < WIN_PAD) win[n + threadIdx.x] = 0.f;            // a group of four at the end of the tokens reads past them
+}
+
+// 16 biases of a lane: rows 32 s + 8 (i / 4) + 4 half + i % 4 of the streamed tile; `at` = 64 window places (bytes) of the tile.
+// BIAS 2: four aligned rows of the tile are neighbours in the window (one row of the grid), BIAS 1: any.
+template <int BIAS>
+__device__ __forceinline__ void read_bias(f32x16& o, const char* win, const int* at, int s, int half, int lane_off) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const int* p = at + 32 * s + 8 * g + 4 * half;
+        if (BIAS == 2) {
+            const float* w = reinterpret_cast<const float*>(win + p[0] + lane_off);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * g + i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * g + i] = *reinterpret_cast<const float*>(win + p[i] + lane_off);
+        }
+    }
+}
+
+// Scores of 16 (lane, streamed row) pairs in units of log2: raw products in, tanh part kept in `th` where asked.
+template <int BIAS, bool CAP>
+__device__ __forceinline__ void to_logits(f32x16& x, f32x16& th, const AttnArgs& a, const char* win, const int* at, int s, int half,
+                                          int lane_off) {
+    f32x16 bias;
+    if (BIAS) read_bias<BIAS>(bias, win, at, s, half, lane_off);
+    if (CAP) {
+        th = x;
+        tanh16(th, a.scale / a.cap);
+        const float f = a.cap * LOG2E;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = BIAS ? th[i] * f + bias[i] : th[i] * f;
+    } else {
+        const float f = a.scale * LOG2E;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = BIAS ? x[i] * f + bias[i] : x[i] * f;
+    }
+}
+
+__device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
+    return a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
+}
+
+// ======================================================================================================= forward
+// LDS: K[2] V[2] tiles | at[2][64] | window.
+// FINE: the probabilities go into the second product as two bf16 terms (16 bits): delta = do . o must be that exact where the
+// fp32 gradient of the table is wanted (with one term it is off by 5e-4, with two by 3e-6); V's fragments serve both.
+template <int D, int BIAS, bool CAP, bool FINE>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    char* kt = smem;
+    char* vt = smem + 2 * TB;
+    int* at = reinterpret_cast<int*>(smem + 4 * TB);
+    float* win = reinterpret_cast<float*>(smem + 4 * TB + 2 * KT * 4);
+
+    const int id = xcd_run(blockIdx.x, gridDim.x);
+    const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int row = qb * BLK + wave * 32 + (lane & 31);
+    const Frags<D> fr(lane);
+
+    bf16x8 qf[KS];
+    {
+        const unsigned short* qp = a.q + b * a.q_sb + (int64_t)min(row, a.Lq - 1) * a.q_sl + h * a.q_sh + 8 * half;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+    }
+    const int len = keys_of(a, b);
+    const int nt = (len + KT - 1) / KT;
+    const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
+    const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
+
+    const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
+    const int pq0 = BIAS ? pos_of(tq0, a.cols) : 0, pq1 = BIAS ? pos_of(tq1, a.cols) : 0;
+    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.cols)) : 0;
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    float m = NEG_INF, l = 0.f;
+
+    Stage<D> sk, sv;
+    auto places = [&](int t) {                                       // window places of tile t's keys, relative to its segment
+        if (BIAS && threadIdx.x < KT) {
+            const int seg0 = pos_of(t / a.seg_tiles * a.seg_tiles * KT, a.cols);
+            at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(min(t * KT + (int)threadIdx.x, a.Lk - 1), a.cols) - seg0);
+        }
+    };
+    if (nt > 0) {
+        sk.load(kp, a.k_sl, 0, len);
+        sv.load(vp, a.v_sl, 0, len);
+        sk.store(kt);
+        sv.store(vt);
+        places(0);
+    }
+    for (int t = 0; t < nt; ++t) {
+        if (BIAS && t % a.seg_tiles == 0) {
+            __syncthreads();                                         // every wave is done with the last window
+            const int last = min((t + a.seg_tiles) * KT, a.Lk) - 1;
+            stage_window<-1>(win, a, h, pq0, pq1, pos_of(t * KT, a.cols), pos_of(last, a.cols));
+        }
+        __syncthreads();
+        const char* kc = kt + (t & 1) * TB;
+        const char* vc = vt + (t & 1) * TB;
+        if (t + 1 < nt) {
+            sk.load(kp, a.k_sl, (t + 1) * KT, len);
+            sv.load(vp, a.v_sl, (t + 1) * KT, len);
+        }
+        f32x16 s[2], th;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) s[u] = mfma(fr.row(kc, 32 * u, ks), qf[ks], s[u]);
+        }
+        float mx = NEG_INF;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            to_logits<BIAS, CAP>(s[u], th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
+            if (t * KT + KT > len) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * KT + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3) >= len) s[u][i] = NEG_INF;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+        }
+        mx = other_half_max(mx);
+        // the reference value follows the maximum only when it falls 2^8 behind: probabilities up to 2^8 lose nothing in bf16 or
+        // in the fp32 sums, and most tiles then skip the rescaling
+        if (__any(mx > m + 8.f)) {
+            const float mn = fmaxf(m, mx);
+            const float al = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.f : mn));
+            m = mn;
+            l *= al;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[d][i] *= al;
+        }
+        const float ms = m == NEG_INF ? 0.f : m;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - ms);
+                l += s[u][i];
+            }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const bf16x8 pf = pack8(s[g >> 1], 8 * (g & 1));
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] = mfma(fr.col(vc, 16 * g, d), pf, o[d]);
+            if (FINE) {
+                f32x16& p = s[g >> 1];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) p[8 * (g & 1) + i] -= (float)pf[i];
+                const bf16x8 pl = pack8(p, 8 * (g & 1));
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = mfma(fr.col(vc, 16 * g, d), pl, o[d]);
+            }
+        }
+        if (t + 1 < nt) {
+            sk.store(kt + ((t + 1) & 1) * TB);
+            sv.store(vt + ((t + 1) & 1) * TB);
+            places(t + 1);
+        }
+    }
+    l = other_half_sum(l);
+    if (row >= a.Lq) return;
+    const float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);       // no key: 0; a NaN stays one
+    if (a.lse && half == 0) a.lse[(int64_t)bh * a.Lq + row] = l == 0.f ? 0.f : m + __builtin_amdgcn_logf(l);
+    const int64_t ob = (((int64_t)b * a.Lq + row) * a.H + h) * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            float f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = o[d][4 * g + i] * il;
+            const u32x2 w = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
+            *reinterpret_cast<u32x2*>(a.out + ob + 32 * d + 8 * g) = w;
+            if (a.out_lo) {                                          // what the rounding dropped: delta needs more than bf16
+                const u32x2 r = {pack_bf16x2(f[0] - bf16_lo(w[0]), f[1] - bf16_hi(w[0])),
+                                 pack_bf16x2(f[2] - bf16_lo(w[1]), f[3] - bf16_hi(w[1]))};
+                *reinterpret_cast<u32x2*>(a.out_lo + ob + 32 * d + 8 * g) = r;
+            }
+        }
+}
+
+// ======================================================================================================= dq, delta and the table
+// Partials of the table's gradient: a pair of tokens (i, j) is known by its distance i - j and by whether the column of i wraps
+// (class 0: dx >= 0, class 1: dx < 0): the two together are the offset.  ds goes through LDS in fp32 and a thread adds up one
+// diagonal of the tile; a diagonal stays with its thread (distance mod 256) over the three tiles it crosses and is then stored
+// once, so no atomics, no clearing and one order of summation.
+// LDS: K[2] V[2] | at[2][64] | ds (64 x 128 fp32, where the table's gradient is wanted) | window.
+template <int D, int BIAS, bool CAP, bool DT>
+__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    char* kt = smem;
+    char* vt = smem + 2 * TB;
+    int* at = reinterpret_cast<int*>(smem + 4 * TB);
+    float* dsl = reinterpret_cast<float*>(smem + 4 * TB + 2 * KT * 4);
+    float* win = dsl + (DT ? KT * BLK : 0);
+
+    const int id = xcd_run(blockIdx.x, gridDim.x);
+    const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int row = qb * BLK + wave * 32 + (lane & 31);
+    const bool live = row < a.Lq;
+    const Frags<D> fr(lane);
+
+    bf16x8 qf[KS], gf[KS];
+    float delta = 0.f;
+    {
+        const int r = min(row, a.Lq - 1);
+        const unsigned short* qp = a.q + b * a.q_sb + (int64_t)r * a.q_sl + h * a.q_sh + 8 * half;
+        const int64_t ob = (((int64_t)b * a.Lq + r) * a.H + h) * D + 8 * half;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+            gf[ks] = *reinterpret_cast<const bf16x8*>(a.d_o + ob + 16 * ks);
+            const bf16x8 ov = *reinterpret_cast<const bf16x8*>(a.o + ob + 16 * ks);
+            const bf16x8 lv = *reinterpret_cast<const bf16x8*>(a.o_lo + ob + 16 * ks);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) delta += (float)gf[ks][i] * ((float)ov[i] + (float)lv[i]);
+        }
+    }
+    delta = other_half_sum(delta);
+    if (live && half == 0) a.delta[(int64_t)bh * a.Lq + row] = delta;
+    if (!live) delta = 0.f;
+    const float lse = live ? a.lse[(int64_t)bh * a.Lq + row] : __builtin_inff();      // a row that is not there has p = 0
+
+    const int len = keys_of(a, b);
+    const int nt = (len + KT - 1) / KT;
+    const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
+    const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
+    const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
+    const int pq0 = BIAS ? pos_of(tq0, a.cols) : 0, pq1 = BIAS ? pos_of(tq1, a.cols) : 0;
+    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.cols)) : 0;
+
+    f32x16 acc[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    float sum0 = 0.f, sum1 = 0.f;                                    // the thread's diagonal, by class
+    // partials of this workgroup, place 0 = the smallest distance it meets
+    float* part = DT ? a.part + (int64_t)id * 2 * a.span : nullptr;
+    const int d_min = tq0 - (nt * KT - 1);
+
+    Stage<D> sk, sv;
+    auto places = [&](int t) {
+        if (BIAS && threadIdx.x < KT) {
+            const int seg0 = pos_of(t / a.seg_tiles * a.seg_tiles * KT, a.cols);
+            at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(min(t * KT + (int)threadIdx.x, a.Lk - 1), a.cols) - seg0);
+        }
+    };
+    if (nt > 0) {
+        sk.load(kp, a.k_sl, 0, len);
+        sv.load(vp, a.v_sl, 0, len);
+        sk.store(kt);
+        sv.store(vt);
+        places(0);
+    }
+    for (int t = 0; t < nt; ++t) {
+        if (BIAS && t % a.seg_tiles == 0) {
+            __syncthreads();
+            const int last = min((t + a.seg_tiles) * KT, a.Lk) - 1;
+            stage_window<-1>(win, a, h, pq0, pq1, pos_of(t * KT, a.cols), pos_of(last, a.cols));
+        }
+        __syncthreads();
+        const char* kc = kt + (t & 1) * TB;
+        const char* vc = vt + (t & 1) * TB;
+        if (t + 1 < nt) {
+            sk.load(kp, a.k_sl, (t + 1) * KT, len);
+            sv.load(vp, a.v_sl, (t + 1) * KT, len);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f32x16 s, dp, th;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                s = mfma(fr.row(kc, 32 * u, ks), qf[ks], s);
+                dp = mfma(fr.row(vc, 32 * u, ks), gf[ks], dp);
+            }
+            to_logits<BIAS, CAP>(s, th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
+            if (t * KT + KT > len) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (t * KT + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3) >= len) s[i] = NEG_INF;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float ds = __builtin_amdgcn_exp2f(s[i] - lse) * (dp[i] - delta);
+                if (DT) dsl[(32 * u + 8 * (i >> 2) + 4 * half + (i & 3)) * BLK + wave * 32 + (lane & 31)] = ds;
+                s[i] = CAP ? ds * (1.f - th[i] * th[i]) : ds;
+            }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bf16x8 pf = pack8(s, 8 * g);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = mfma(fr.col(kc, 32 * u + 16 * g, d), pf, acc[d]);
+            }
+        }
+        if (t + 1 < nt) {
+            sk.store(kt + ((t + 1) & 1) * TB);
+            sv.store(vt + ((t + 1) & 1) * TB);
+            places(t + 1);
+        }
+        if (DT) {
+            __syncthreads();
+            const int k0 = t * KT, lo = tq0 - k0 - (KT - 1);         // smallest distance of this tile
+            const int w = ((int)threadIdx.x - lo) & 255;
+            const int c = w - (KT - 1), dist = lo + w;               // column of the tile = row + c
+            if (c < BLK) {
+                const int k_lo = max(0, -c), k_hi = min(KT - 1, BLK - 1 - c);
+                const float* p = dsl + k_lo * (BLK + 1) + c;
+                if (a.rows == 1) {
+                    for (int k = k_lo; k <= k_hi; ++k, p += BLK + 1) sum0 += *p;
+                } else {
+                    int r = dist % a.cols;
+                    r += r < 0 ? a.cols : 0;
+                    int x = (k0 + k_lo) % a.cols + r - a.cols;       // >= 0: the column of i wraps
+                    const int wrap = r;
+                    for (int k = k_lo; k <= k_hi; ++k, p += BLK + 1) {
+                        const float v = *p;
+                        if (x >= 0) sum1 += v;
+                        else sum0 += v;
+                        ++x;
+                        if (x == wrap) x -= a.cols;                  // the key's own row ends
+                    }
+                }
+                if (c >= KT || t + 1 == nt) {                        // the diagonal leaves the workgroup's rows
+                    part[dist - d_min] = sum0;
+                    part[a.span + dist - d_min] = sum1;
+                    sum0 = sum1 = 0.f;
+                }
+            }
+        }
+    }
+    if (!live) return;
+    unsigned short* qo = a.dq + b * a.dq_sb + (int64_t)row * a.dq_sl + h * a.dq_sh + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const u32x2 w = {pack_bf16x2(acc[d][4 * g] * a.scale, acc[d][4 * g + 1] * a.scale),
+                             pack_bf16x2(acc[d][4 * g + 2] * a.scale, acc[d][4 * g + 3] * a.scale)};
+            *reinterpret_cast<u32x2*>(qo + 32 * d + 8 * g) = w;
+        }
+}
+
+// ---- the table's gradient from the partials: by distance and class first, then by bucket.
+// by_dist (H, 2, 2 n - 1): grid (distances / 256, 2 classes x H); a thread adds its distance over samples and query blocks.
+__global__ __launch_bounds__(256) void attn_dist_kernel(AttnArgs a, float* by_dist, int n_dist, int d0) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    const int cls = blockIdx.y & 1, h = blockIdx.y >> 1;
+    if (i >= n_dist) return;
+    const int dist = i + d0;
+    float s = 0.f;
+    for (int b = 0; b < a.B; ++b) {
+        const int nt = (keys_of(a, b) + KT - 1) / KT;
+        if (nt == 0) continue;
+        for (int qb = 0; qb < a.n_qb; ++qb) {
+            const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * KT - 1));
+            if (place < 0 || dist > tq0 + BLK - 1) continue;
+            s += a.part[((int64_t)((b * a.H + h) * a.n_qb + qb) * 2 + cls) * a.span + place];
+        }
+    }
+    by_dist[((int64_t)h * 2 + cls) * n_dist + i] = s;
+}
+
+// dtable[h][u] = sum over the offsets of bucket u (order[start[u]] .. ): grid (n_buckets, H), a wave each.
+__global__ __launch_bounds__(64) void attn_bucket_kernel(AttnArgs a, const float* by_dist, const int* order, const int* start, int n_dist,
+                                                         int d0) {
+    const int u = blockIdx.x, h = blockIdx.y, w = 2 * a.cols - 1;
+    const float* src = by_dist + (int64_t)h * 2 * n_dist;
+    float s = 0.f;
+    for (int e = start[u] + (int)threadIdx.x; e < start[u + 1]; e += 64) {
+        const int off = order[e], dy = off / w - (a.rows - 1), dx = off % w - (a.cols - 1);
+        const int place = dy * a.cols + dx - d0;
+        const int cls = a.rows > 1 && dx < 0 ? 1 : 0;
+        if (place >= 0 && place < n_dist) s += src[(int64_t)cls * n_dist + place];
+    }
+    s = wave_sum(s);
+    if (threadIdx.x == 0) a.dtable[(int64_t)h * a.n_buckets + u] = s;
+}
+
+// ======================================================================================================= dk, dv
+// A workgroup owns 128 keys of one key / value head and streams the queries of every head that shares it: scores here are
+// queries x keys, a lane holds one key.  No sum leaves the workgroup.
+// LDS: Q[2] dO[2] | at[2][64] | lse[2][64] | delta[2][64] | window.
+template <int D, int BIAS, bool CAP>
+__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    char* qt = smem;
+    char* gt = smem + 2 * TB;
+    int* at = reinterpret_cast<int*>(smem + 4 * TB);
+    float* ls = reinterpret_cast<float*>(at + 2 * KT);
+    float* dl = ls + 2 * KT;
+    float* win = dl + 2 * KT;
+
+    const int id = xcd_run(blockIdx.x, gridDim.x);
+    const int kb = id % a.n_kb, bk = id / a.n_kb, hk = bk % a.Hkv, b = bk / a.Hkv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
+    const int key = kb * BLK + wave * 32 + (lane & 31);
+    const Frags<D> fr(lane);
+    const int len = keys_of(a, b);
+
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
+
+    if (kb * BLK < len && a.Lq > 0) {
+        bf16x8 kf[KS], vf[KS];
+        {
+            const int r = min(key, len - 1);                         // keys beyond the length repeat the last one; their sums are dropped
+            const unsigned short* kp = a.k + b * a.k_sb + (int64_t)r * a.k_sl + hk * a.k_sh + 8 * half;
+            const unsigned short* vp = a.v + b * a.v_sb + (int64_t)r * a.v_sl + hk * a.v_sh + 8 * half;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                kf[ks] = *reinterpret_cast<const bf16x8*>(kp + 16 * ks);
+                vf[ks] = *reinterpret_cast<const bf16x8*>(vp + 16 * ks);
+            }
+        }
+        const int tk0 = kb * BLK, tk1 = min(kb * BLK + BLK, a.Lk) - 1;
+        const int pk0 = BIAS ? pos_of(tk0, a.cols) : 0, pk1 = BIAS ? pos_of(tk1, a.cols) : 0;
+        const int lane_off = BIAS ? 4 * (pk1 - pos_of(min(key, tk1), a.cols)) : 0;
+        const int nqt = (a.Lq + KT - 1) / KT, nt = nqt * a.rep;
+
+        Stage<D> sq, sg;
+        float next_l = 0.f, next_d = 0.f;
+        auto load = [&](int t) {
+            const int h = hk * a.rep + t / nqt, r0 = t % nqt * KT;
+            sq.load(a.q + b * a.q_sb + h * a.q_sh, a.q_sl, r0, a.Lq);
+            sg.load(a.d_o + ((int64_t)b * a.Lq * a.H + h) * D, (int64_t)a.H * D, r0, a.Lq);
+            if (threadIdx.x < KT) {
+                const int r = r0 + threadIdx.x;
+                const int64_t at_row = (int64_t)(b * a.H + h) * a.Lq + r;
+                next_l = r < a.Lq ? a.lse[at_row] : __builtin_inff();
+                next_d = r < a.Lq ? a.delta[at_row] : 0.f;
+            }
+        };
+        auto store = [&](int t) {
+            sq.store(qt + (t & 1) * TB);
+            sg.store(gt + (t & 1) * TB);
+            if (threadIdx.x < KT) {
+                ls[(t & 1) * KT + threadIdx.x] = next_l;
+                dl[(t & 1) * KT + threadIdx.x] = next_d;
+                if (BIAS) {
+                    const int tt = t % nqt, seg0 = a.q_start + tt / a.seg_tiles * a.seg_tiles * KT;
+                    const int tok = a.q_start + min(tt * KT + (int)threadIdx.x, a.Lq - 1);
+                    at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(tok, a.cols) - pos_of(seg0, a.cols));
+                }
+            }
+        };
+        load(0);
+        store(0);
+        for (int t = 0; t < nt; ++t) {
+            const int tt = t % nqt;
+            if (BIAS && tt % a.seg_tiles == 0) {
+                __syncthreads();
+                const int last = a.q_start + min((tt + a.seg_tiles) * KT, a.Lq) - 1;
+                stage_window<1>(win, a, hk * a.rep + t / nqt, pk0, pk1, pos_of(a.q_start + tt * KT, a.cols), pos_of(last, a.cols));
+            }
+            __syncthreads();
+            const char* qc = qt + (t & 1) * TB;
+            const char* gc = gt + (t & 1) * TB;
+            const float* lc = ls + (t & 1) * KT;
+            const float* dc = dl + (t & 1) * KT;
+            if (t + 1 < nt) load(t + 1);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f32x16 s, dp, th;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    s = mfma(fr.row(qc, 32 * u, ks), kf[ks], s);
+                    dp = mfma(fr.row(gc, 32 * u, ks), vf[ks], dp);
+                }
+                to_logits<BIAS, CAP>(s, th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lc + 32 * u + 8 * g + 4 * half);
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(dc + 32 * u + 8 * g + 4 * half);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int e = 4 * g + i;
+                        s[e] = __builtin_amdgcn_exp2f(s[e] - l4[i]);
+                        dp[e] = s[e] * (dp[e] - d4[i]);
+                        if (CAP) dp[e] *= 1.f - th[e] * th[e];
+                    }
+                }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const bf16x8 pf = pack8(s, 8 * g), df = pack8(dp, 8 * g);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) {
+                        dv[d] = mfma(fr.col(gc, 32 * u + 16 * g, d), pf, dv[d]);
+                        dk[d] = mfma(fr.col(qc, 32 * u + 16 * g, d), df, dk[d]);
+                    }
+                }
+            }
+            if (t + 1 < nt) store(t + 1);
+        }
+    }
+    if (key >= a.Lk) return;
+    const bool in = key < len;
+    unsigned short* ko = a.dk + b * a.dk_sb + (int64_t)key * a.dk_sl + hk * a.dk_sh + 4 * half;
+    unsigned short* vo = a.dv + b * a.dv_sb + (int64_t)key * a.dv_sl + hk * a.dv_sh + 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            u32x2 w = {pack_bf16x2(dk[d][4 * g] * a.scale, dk[d][4 * g + 1] * a.scale),
+                       pack_bf16x2(dk[d][4 * g + 2] * a.scale, dk[d][4 * g + 3] * a.scale)};
+            u32x2 x = {pack_bf16x2(dv[d][4 * g], dv[d][4 * g + 1]), pack_bf16x2(dv[d][4 * g + 2], dv[d][4 * g + 3])};
+            if (!in) w = x = u32x2{0, 0};
+            *reinterpret_cast<u32x2*>(ko + 32 * d + 8 * g) = w;
+            *reinterpret_cast<u32x2*>(vo + 32 * d + 8 * g) = x;
+        }
+}
+
+// ======================================================================================================= host side
+// Tiles of 64 streamed tokens whose bias window, next to 128 owned ones, fits WIN_FLOATS (0: not even one does).
+int span_of(int n, int rows, int cols) {                              // the most P(last) - P(first) can be over n consecutive tokens
+    if (n <= 1) return 0;
+    int64_t crossings = rows > 1 ? (n - 2 + cols) / cols : 0;
+    if (crossings > rows - 1) crossings = rows - 1;
+    const int64_t s = (n - 1) + crossings * (cols - 1);
+    return s > (1 << 30) ? 1 << 30 : (int)s;
+}
+int segment_tiles(int owned, int streamed, int rows, int cols) {
+    const int own = span_of(owned < BLK ? owned : BLK, rows, cols);
+    const int tiles = ceil_div(streamed, KT);
+    int lo = 0;
+    for (int t = tiles; t > 0; t = t > 64 ? t / 2 : t - 1) {
+        const int64_t n = (int64_t)t * KT < streamed ? (int64_t)t * KT : streamed;
+        if ((int64_t)own + span_of((int)n, rows, cols) + 1 <= WIN_FLOATS) { lo = t; break; }
+    }
+    return lo;
+}
+size_t window_bytes(int owned, int streamed, int rows, int cols, int seg) {
+    const int64_t n = (int64_t)seg * KT < streamed ? (int64_t)seg * KT : streamed;
+    return 4 * ((size_t)span_of(owned < BLK ? owned : BLK, rows, cols) + span_of((int)n, rows, cols) + 1 + WIN_PAD);
+}
+
+int check_desc(const rgbd_attn_desc* d, const char* who) {
+    RGBD_REQUIRE(d != nullptr, "%s: null descriptor", who);
+    RGBD_REQUIRE(d->B >= 0 && d->H > 0 && d->Hkv > 0 && d->Lq >= 0 && d->Lk >= 0 && d->H % d->Hkv == 0,
+                 "%s: bad sizes B=%d H=%d Hkv=%d Lq=%d Lk=%d (Hkv must divide H)", who, d->B, d->H, d->Hkv, d->Lq, d->Lk);
+    RGBD_REQUIRE(d->D == 32 || d->D == 64 || d->D == 128, "%s: head size %d is not one of 32, 64, 128", who, d->D);
+    RGBD_REQUIRE(d->Lq < (1 << 24) && d->Lk < (1 << 24) && (int64_t)d->B * d->H * (ceil_div(d->Lq, BLK) + ceil_div(d->Lk, BLK)) < (1 << 30),
+                 "%s: too many tokens", who);
+    RGBD_REQUIRE(d->cap >= 0.f, "%s: cap must not be negative", who);
+    const int64_t st[9] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh};
+    for (int i = 0; i < 9; ++i) RGBD_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    RGBD_REQUIRE((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) == 0, "%s: q, k, v must be 16-byte aligned", who);
+    if (d->table) {
+        RGBD_REQUIRE(d->map != nullptr && d->n_buckets > 0, "%s: a bias table needs its bucket map", who);
+        RGBD_REQUIRE(d->rows > 0 && d->cols > 0 && (int64_t)d->rows * d->cols < (1 << 24), "%s: bad grid %d x %d", who, d->rows, d->cols);
+        RGBD_REQUIRE(d->rows == 1 || d->cols <= 1024, "%s: a grid of more than one row has at most 1024 columns, got %d", who, d->cols);
+        RGBD_REQUIRE(d->q_start >= 0 && (int64_t)d->q_start + d->Lq <= (int64_t)d->rows * d->cols && d->Lk <= (int64_t)d->rows * d->cols,
+                     "%s: tokens outside the %d x %d grid (q_start=%d Lq=%d Lk=%d)", who, d->rows, d->cols, d->q_start, d->Lq, d->Lk);
+    }
+    return 0;
+}
+
+AttnArgs args_of(const rgbd_attn_desc* d) {
+    AttnArgs a{};
+    a.q = (const unsigned short*)d->q; a.k = (const unsigned short*)d->k; a.v = (const unsigned short*)d->v;
+    a.q_sb = d->q_sb; a.q_sl = d->q_sl; a.q_sh = d->q_sh;
+    a.k_sb = d->k_sb; a.k_sl = d->k_sl; a.k_sh = d->k_sh;
+    a.v_sb = d->v_sb; a.v_sl = d->v_sl; a.v_sh = d->v_sh;
+    a.table = d->table; a.map = d->map; a.lengths = d->lengths;
+    a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.rep = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
+    a.rows = d->table ? d->rows : 1; a.cols = d->table ? d->cols : 1 << 24; a.q_start = d->table ? d->q_start : 0;
+    a.n_buckets = d->n_buckets;
+    a.scale = d->scale; a.cap = d->cap;
+    a.n_qb = ceil_div(d->Lq, BLK); a.n_kb = ceil_div(d->Lk, BLK);
+    a.lse = d->lse;
+    return a;
+}
+
+// 0 no bias; 2 four aligned tokens of a streamed tile share a grid row; 1 they may not.
+int bias_mode(const rgbd_attn_desc* d, int first) {
+    if (!d->table) return 0;
+    return d->rows == 1 || (d->cols % 4 == 0 && first % 4 == 0) ? 2 : 1;
+}
+
+#define BY_BIAS_CAP(KERNEL, D, ...)                                                                                     \
+    do {                                                                                                                \
+        if (cap) {                                                                                                      \
+            if (bias == 0) LAUNCH((KERNEL<D, 0, true __VA_ARGS__>));                                                    \
+            else if (bias == 1) LAUNCH((KERNEL<D, 1, true __VA_ARGS__>));                                               \
+            else LAUNCH((KERNEL<D, 2, true __VA_ARGS__>));                                                              \
+        } else {                                                                                                        \
+            if (bias == 0) LAUNCH((KERNEL<D, 0, false __VA_ARGS__>));                                                   \
+            else if (bias == 1) LAUNCH((KERNEL<D, 1, false __VA_ARGS__>));                                              \
+            else LAUNCH((KERNEL<D, 2, false __VA_ARGS__>));                                                             \
+        }                                                                                                               \
+    } while (0)
+#define LAUNCH(K)                                                                                                       \
+    do {                                                                                                                \
+        if (!rgbd_reserve_lds((const void*)&K, (int)lds)) { rgbd_set_error("attention: cannot reserve %d bytes of LDS", (int)lds); return -2; } \
+        hipLaunchKernelGGL(K, dim3(grid), dim3(256), lds, s, a);                                                        \
+    } while (0)
+
+template <int D> int launch_fwd(const AttnArgs& a, int bias, bool cap, bool fine, unsigned grid, size_t lds, hipStream_t s) {
+    if (!fine) { BY_BIAS_CAP(attn_fwd_kernel, D, , false); return 0; }
+    if (cap) { if (bias == 1) LAUNCH((attn_fwd_kernel<D, 1, true, true>)); else LAUNCH((attn_fwd_kernel<D, 2, true, true>)); }
+    else { if (bias == 1) LAUNCH((attn_fwd_kernel<D, 1, false, true>)); else LAUNCH((attn_fwd_kernel<D, 2, false, true>)); }
+    return 0;
+}
+template <int D> int launch_dq(const AttnArgs& a, int bias, bool cap, bool dt, unsigned grid, size_t lds, hipStream_t s) {
+    if (!dt) { BY_BIAS_CAP(attn_dq_kernel, D, , false); return 0; }
+    if (cap) { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, true, true>)); else LAUNCH((attn_dq_kernel<D, 2, true, true>)); }
+    else { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, false, true>)); else LAUNCH((attn_dq_kernel<D, 2, false, true>)); }
+    return 0;
+}
+template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned grid, size_t lds, hipStream_t s) {
+    BY_BIAS_CAP(attn_dkv_kernel, D);
+    return 0;
+}
+
+struct BwdSizes { int64_t delta, part, by_dist; int span, n_dist, d0; };
+BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
+    BwdSizes z{};
+    z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
+    if (dt && d->Lq > 0 && d->Lk > 0) {
+        const int n_qb = ceil_div(d->Lq, BLK);
+        z.span = ceil_div(d->Lk, KT) * KT + BLK;
+        z.part = (int64_t)d->B * d->H * n_qb * 2 * z.span;
+        z.d0 = d->q_start - (ceil_div(d->Lk, KT) * KT - 1);           // distances from there to q_start + n_qb * BLK - 1
+        z.n_dist = d->q_start + n_qb * BLK - z.d0;
+        z.by_dist = (int64_t)d->H * 2 * z.n_dist;
+    }
+    return z;
+}
+
+}  // namespace
+
+extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, void* stream) {
+    if (check_desc(d, "rgbd_attention_fwd")) return -1;
+    if (d->B == 0 || d->Lq == 0) return 0;
+    RGBD_REQUIRE(d->q && o && (d->Lk == 0 || (d->k && d->v)), "rgbd_attention_fwd: null pointer");
+    RGBD_REQUIRE((((uintptr_t)o | (uintptr_t)o_lo) & 15) == 0, "rgbd_attention_fwd: outputs must be 16-byte aligned");
+    AttnArgs a = args_of(d);
+    a.out = (unsigned short*)o;
+    a.out_lo = (unsigned short*)o_lo;
+    const int bias = bias_mode(d, 0);
+    size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4;
+    if (bias && d->Lk > 0) {
+        a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols);
+        RGBD_REQUIRE(a.seg_tiles > 0, "rgbd_attention_fwd: the bias of one tile does not fit (%d x %d grid)", a.rows, a.cols);
+        lds += window_bytes(d->Lq, d->Lk, a.rows, a.cols, a.seg_tiles);
+    }
+    const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
+    hipStream_t s = (hipStream_t)stream;
+    const bool cap = d->cap > 0.f;
+    const bool fine = d->fine && bias;
+    const int rc = d->D == 32   ? launch_fwd<32>(a, bias, cap, fine, grid, lds, s)
+                   : d->D == 64 ? launch_fwd<64>(a, bias, cap, fine, grid, lds, s)
+                                : launch_fwd<128>(a, bias, cap, fine, grid, lds, s);
+    if (rc) return rc;
+    RGBD_CHECK_LAUNCH("rgbd_attention_fwd");
+    return 0;
+}
+
+extern "C" int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table) {
+    if (check_desc(d, "rgbd_attention_bwd_workspace")) return -1;
+    const BwdSizes z = bwd_sizes(d, want_table && d->table);
+    return z.delta + z.part + z.by_dist + 4;
+}
+
+extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream) {
+    const char* who = "rgbd_attention_bwd";
+    if (check_desc(d, who)) return -1;
+    RGBD_REQUIRE(g != nullptr, "%s: null gradient descriptor", who);
+    const bool dt = g->dtable != nullptr;
+    RGBD_REQUIRE(!dt || (d->table && g->order && g->start), "%s: the table's gradient needs the table and its buckets' offsets", who);
+    hipStream_t s = (hipStream_t)stream;
+    const bool empty = d->B == 0 || d->Lq == 0 || d->Lk == 0;
+    if (dt && empty) {
+        const hipError_t e = rgbd_zero_async(g->dtable, (size_t)d->H * d->n_buckets * 4, s);
+        RGBD_REQUIRE(e == hipSuccess, "%s: %s", who, hipGetErrorString(e));
+    }
+    if (d->B == 0) return 0;
+    RGBD_REQUIRE(workspace && (d->Lq == 0 || (d->q && d->lse && g->d_o && g->o && g->o_lo && g->dq)) &&
+                 (d->Lk == 0 || (d->k && d->v && g->dk && g->dv)), "%s: null pointer", who);
+    const int64_t st[9] = {g->dq_sb, g->dq_sl, g->dq_sh, g->dk_sb, g->dk_sl, g->dk_sh, g->dv_sb, g->dv_sl, g->dv_sh};
+    for (int i = 0; i < 9; ++i) RGBD_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    RGBD_REQUIRE((((uintptr_t)g->d_o | (uintptr_t)g->o | (uintptr_t)g->o_lo | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv |
+                   (uintptr_t)workspace) & 15) == 0, "%s: buffers must be 16-byte aligned", who);
+    AttnArgs a = args_of(d);
+    a.d_o = (const unsigned short*)g->d_o; a.o = (const unsigned short*)g->o; a.o_lo = (const unsigned short*)g->o_lo;
+    a.dq = (unsigned short*)g->dq; a.dk = (unsigned short*)g->dk; a.dv = (unsigned short*)g->dv;
+    a.dq_sb = g->dq_sb; a.dq_sl = g->dq_sl; a.dq_sh = g->dq_sh;
+    a.dk_sb = g->dk_sb; a.dk_sl = g->dk_sl; a.dk_sh = g->dk_sh;
+    a.dv_sb = g->dv_sb; a.dv_sl = g->dv_sl; a.dv_sh = g->dv_sh;
+    a.dtable = g->dtable;
+    const BwdSizes z = bwd_sizes(d, dt);
+    a.delta = workspace;
+    a.part = workspace + z.delta;
+    a.span = z.span;
+    float* by_dist = a.part + z.part;
+    const bool cap = d->cap > 0.f;
+
+    if (d->Lq > 0) {
+        const int bias = bias_mode(d, 0);
+        size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4 + (dt ? KT * BLK * 4 : 0);
+        a.seg_tiles = 1;
+        if (bias && d->Lk > 0) {
+            a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols);
+            RGBD_REQUIRE(a.seg_tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
+            lds += window_bytes(d->Lq, d->Lk, a.rows, a.cols, a.seg_tiles);
+        }
+        const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
+        const int rc = d->D == 32 ? launch_dq<32>(a, bias, cap, dt, grid, lds, s) : d->D == 64 ? launch_dq<64>(a, bias, cap, dt, grid, lds, s)
+                                                                                               : launch_dq<128>(a, bias, cap, dt, grid, lds, s);
+        if (rc) return rc;
+        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dq)");
+    }
+    if (dt && !empty) {
+        hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 256), 2 * a.H), dim3(256), 0, s, a, by_dist, z.n_dist, z.d0);
+        hipLaunchKernelGGL(attn_bucket_kernel, dim3(a.n_buckets, a.H), dim3(64), 0, s, a, by_dist, g->order, g->start, z.n_dist, z.d0);
+        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
+    }
+    if (d->Lk > 0) {
+        const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
+        size_t lds = 4 * KT * 2 * d->D + 6 * KT * 4;
+        a.seg_tiles = 1;
+        if (bias) {
+            a.seg_tiles = segment_tiles(d->Lk, d->Lq, a.rows, a.cols);
+            RGBD_REQUIRE(a.seg_tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
+            lds += window_bytes(d->Lk, d->Lq, a.rows, a.cols, a.seg_tiles);
+        }
+        const unsigned grid = (unsigned)a.B * a.Hkv * a.n_kb;
+        const int rc = d->D == 32 ? launch_dkv<32>(a, bias, cap, grid, lds, s) : d->D == 64 ? launch_dkv<64>(a, bias, cap, grid, lds, s)
+                                                                                            : launch_dkv<128>(a, bias, cap, grid, lds, s);
+        if (rc) return rc;
+        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dk, dv)");
+    }
+    return 0;
+}

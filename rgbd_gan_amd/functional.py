@@ -14,6 +14,7 @@ Layout: activations are NHWC bf16 tensors of shape (B,H,W,C); master weights are
 import contextlib
 import os
 
+import numpy as np
 import torch
 import torch.nn.functional as F
 
@@ -1667,3 +1668,151 @@ class _FoldView(torch.autograd.Function):
 def fold_weight(W, mode, Cop, Cip):
     """Master conv parameter -> the weight the 2-D conv engine packs (kernels.fold_weight), differentiable."""
     return _FoldWeight.apply(W, mode, Cop, Cip)
+
+
+# ---- group norm and attention over feature maps
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, beta, groups, eps, act, slope):
+        y, mean, rstd = kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)
+        ctx.groups, ctx.act, ctx.slope = groups, act, slope
+        ctx.save_for_backward(x, gamma, beta, mean, rstd)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, gamma, beta, mean, rstd = ctx.saved_tensors
+        dx, dgamma, dbeta = kernels.group_norm_bwd(x, dy.contiguous(), gamma, beta, mean, rstd, ctx.groups, ctx.act, ctx.slope)
+        return dx, dgamma, dbeta, None, None, None, None
+
+
+def group_norm(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
+    """act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and variance over each sample's groups of C / groups neighbouring
+    channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu"."""
+    return _GroupNorm.apply(x.contiguous(), gamma.contiguous(), beta.contiguous(), groups, eps, act, slope)
+
+
+class RelativeBuckets:
+    """Which entry of a learned bias table each offset between two tokens of a rows x cols grid reads.
+
+    offsets: (2 rows - 1, 2 cols - 1) integers in [0, n_buckets); offsets[dy + rows - 1, dx + cols - 1] is the bucket of a query
+    dy rows below and dx columns right of its key.  Built once for a feature map's size; holds the map and, for the table's
+    gradient, each bucket's offsets on the device."""
+
+    def __init__(self, offsets, n_buckets=None, device="cuda"):
+        m = offsets.detach().cpu().numpy() if torch.is_tensor(offsets) else np.asarray(offsets)
+        if m.ndim != 2 or m.shape[0] % 2 != 1 or m.shape[1] % 2 != 1 or not np.issubdtype(m.dtype, np.integer):
+            raise ValueError(f"RelativeBuckets: offsets must be integers of shape (2 rows - 1, 2 cols - 1), got {m.dtype} {m.shape}")
+        n = int(m.max()) + 1 if n_buckets is None else int(n_buckets)
+        if m.min() < 0 or m.max() >= n:
+            raise ValueError(f"RelativeBuckets: bucket numbers must lie in [0, {n}), got {m.min()} .. {m.max()}")
+        self.rows, self.cols, self.n_buckets = (m.shape[0] + 1) // 2, (m.shape[1] + 1) // 2, n
+        flat = m.reshape(-1)
+        to = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(device)
+        self.map = to(flat)
+        self.order = to(np.argsort(flat, kind="stable"))
+        self.start = to(np.concatenate([[0], np.cumsum(np.bincount(flat, minlength=n))]))
+
+    @classmethod
+    def log(cls, rows, cols, per_axis=15, max_distance=64, device="cuda"):
+        """per_axis (odd) buckets along each axis, the sign kept: one each for the nearest distances, logarithmic up to
+        max_distance, the last for all beyond; a grid of one row has one axis."""
+        if per_axis < 3 or per_axis % 2 != 1:
+            raise ValueError(f"RelativeBuckets.log: per_axis must be odd and at least 3, got {per_axis}")
+
+        def axis(n):
+            half = (per_axis - 1) // 2
+            near = max(1, half // 2)
+            d = np.arange(-(n - 1), n)
+            a = np.abs(d)
+            far = near + np.floor(np.log(np.maximum(a, near) / near) / np.log(max(max_distance, near + 1) / near) * (half - near))
+            return half + np.sign(d) * np.minimum(np.where(a <= near, a, far.astype(np.int64)), half)
+
+        x = axis(cols)
+        if rows == 1:
+            return cls(x[None, :].astype(np.int64), per_axis, device)
+        return cls((axis(rows)[:, None] * per_axis + x[None, :]).astype(np.int64), per_axis ** 2, device)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, lengths, spec):
+        o, o_lo, lse = kernels.attention_fwd(q, k, v, table, lengths=lengths, keep=True, fine=ctx.needs_input_grad[3], **spec)
+        ctx.spec = spec
+        ctx.save_for_backward(q, k, v, table, lengths, o, o_lo, lse)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o):
+        q, k, v, table, lengths, o, o_lo, lse = ctx.saved_tensors
+        dq, dk, dv, dtable = kernels.attention_bwd(q, k, v, d_o.contiguous(), o, o_lo, lse, table, lengths=lengths,
+                                                   want_table=ctx.needs_input_grad[3], **ctx.spec)
+        return dq, dk, dv, dtable, None, None
+
+
+def _packed_views(qkv, heads, kv_heads, D):
+    B, N, _ = qkv.shape
+    view = lambda lo, n: qkv[:, :, lo * D:(lo + n) * D].unflatten(2, (n, D))
+    return view(0, heads), view(heads, kv_heads), view(heads + kv_heads, kv_heads)
+
+
+class _AttentionPacked(torch.autograd.Function):
+    """The three gradients are written into one tensor of the packed layout."""
+
+    @staticmethod
+    def forward(ctx, qkv, table, lengths, layout, spec):
+        o, o_lo, lse = kernels.attention_fwd(*_packed_views(qkv, *layout), table, lengths=lengths, keep=True,
+                                            fine=ctx.needs_input_grad[1], **spec)
+        ctx.layout, ctx.spec = layout, spec
+        ctx.save_for_backward(qkv, table, lengths, o, o_lo, lse)
+        return o
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o):
+        qkv, table, lengths, o, o_lo, lse = ctx.saved_tensors
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dtable = kernels.attention_bwd(*_packed_views(qkv, *ctx.layout), d_o.contiguous(), o, o_lo, lse, table, lengths=lengths,
+                                       out=_packed_views(dqkv, *ctx.layout), want_table=ctx.needs_input_grad[1], **ctx.spec)[3]
+        return dqkv, dtable, None, None, None
+
+
+def _attention_spec(buckets, scale, cap, q_start):
+    return dict(buckets=buckets, scale=scale, cap=float(cap or 0.0), q_start=int(q_start))
+
+
+def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=None, q_start=0):
+    """softmax(cap tanh(scale q k^T / cap) + bias) v, every row over its sample's first lengths[b] keys (0 where there are none).
+
+    q (B, Lq, H, D), k, v (B, Lk, Hkv, D) bf16 at any strides, D 32, 64 or 128, H a multiple of Hkv (query head h reads key / value
+    head h // (H // Hkv)); scale defaults to D ** -0.5, cap 0 leaves scores uncapped; lengths (B,) int32 on the device.
+    table (H, n_buckets) fp32 with `buckets` (RelativeBuckets): the bias table[h, bucket of the offset], query i at token
+    q_start + i of the grid, key j at token j.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table."""
+    spec = _attention_spec(buckets, scale, cap, q_start)
+    q, k, v = (t if t.dim() != 4 or kernels.attention_readable(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    table = table.contiguous() if table is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
+        return _Attention.apply(q, k, v, table, lengths, spec)
+    return kernels.attention_fwd(q, k, v, table, lengths=lengths, **spec)[0]
+
+
+def attention_packed(qkv, heads, kv_heads=None, table=None, buckets=None, scale=None, cap=0.0, lengths=None):
+    """attention() of a projection's output: qkv (B, N, (heads + 2 kv_heads) D) or (B, H, W, ...) bf16, a token's channels being its
+    query heads, then its key heads, then its value heads; kv_heads defaults to heads.  -> (B, N, heads, D)."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if qkv.dim() == 4:
+        qkv = qkv.flatten(1, 2)
+    if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
+        raise RuntimeError(f"attention_packed: {tuple(qkv.shape)} does not split into {heads} + 2 x {kv_heads} heads")
+    layout = (heads, kv_heads, qkv.shape[2] // (heads + 2 * kv_heads))
+    spec = _attention_spec(buckets, scale, cap, 0)
+    if not kernels.attention_readable(qkv.unsqueeze(2)):
+        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    table = table.contiguous() if table is not None else None
+    lengths = lengths.contiguous() if lengths is not None else None
+    if torch.is_grad_enabled() and (qkv.requires_grad or (table is not None and table.requires_grad)):
+        return _AttentionPacked.apply(qkv, table, lengths, layout, spec)
+    return kernels.attention_fwd(*_packed_views(qkv, *layout), table, lengths=lengths, **spec)[0]

@@ -1535,3 +1535,217 @@ def fold_weight(src, mode, Co, Ci, K, Cop, Cip, adjoint=False, out=None):
     _lib.check(_lib.load().rgbd_fold_weight_f32(_ptr(src), _ptr(dst), mode, Co, Ci, K, Cop, Cip, flag, _stream()),
                "rgbd_fold_weight_f32")
     return dst
+
+
+# ------------------------------------------------------------------ group norm, attention
+ACTS = {None: 0, "none": 0, "lrelu": 1, "silu": 2}
+
+
+def _chk_device(what, *tensors):
+    """Every tensor on the current device: the launch goes to that device's current stream."""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise RuntimeError(f"{what}: tensor on {t.device}, current device is cuda:{cur}")
+
+
+def _gn_sizes(x, gamma, beta, groups, act):
+    if not torch.is_tensor(x) or x.dim() < 2:
+        raise RuntimeError("group_norm: x must have a batch and a channel axis, (B, ..., C)")
+    if x.dtype not in (BF16, F32):
+        raise RuntimeError(f"group_norm: x must be bf16 or fp32, got {x.dtype}")
+    if act not in ACTS:
+        raise RuntimeError(f"group_norm: act must be one of {sorted(k for k in ACTS if k)}, got {act!r}")
+    C = x.shape[-1]
+    groups = int(groups)
+    if groups < 1 or C < 1 or C % groups:
+        raise RuntimeError(f"group_norm: {groups} groups do not divide {C} channels")
+    for t, name in ((gamma, "gamma"), (beta, "beta")):
+        if tuple(t.shape) != (C,):
+            raise RuntimeError(f"group_norm: {name} must have shape ({C},), got {tuple(t.shape)}")
+    N = 1
+    for n in x.shape[1:-1]:
+        N *= n
+    _chk(x, x.dtype, "x"); _chk(gamma, F32, "gamma"); _chk(beta, F32, "beta")
+    _chk_device("group_norm", x, gamma, beta)
+    return x.shape[0], N, C, groups, 0 if x.dtype == BF16 else 1
+
+
+def _gn_workspace(sizes, backward, device):
+    n = _lib.load().rgbd_group_norm_workspace(*sizes, int(backward))
+    if n < 0:
+        _lib.check(-1, "rgbd_group_norm_workspace")
+    return torch.empty(n, dtype=F32, device=device)
+
+
+def group_norm_fwd(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
+    """x (B, ..., C) bf16 or fp32, gamma, beta (C,) fp32 -> y like x, mean, rstd (B, groups) fp32."""
+    B, N, C, groups, dt = sizes = _gn_sizes(x, gamma, beta, groups, act)
+    if not eps >= 0:
+        raise RuntimeError(f"group_norm: eps must not be negative, got {eps}")
+    y = torch.empty_like(x)
+    stats = torch.empty(2, B, groups, dtype=F32, device=x.device)
+    ws = _gn_workspace(sizes, False, x.device)
+    rc = _timed("gn_fwd", 0, 2 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_fwd(
+        _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(stats[0]), _ptr(stats[1]), _ptr(ws), B, N, C, groups, dt, ACTS[act],
+        float(eps), float(slope), _stream()))
+    _lib.check(rc, "rgbd_group_norm_fwd")
+    return y, stats[0], stats[1]
+
+
+def group_norm_bwd(x, dy, gamma, beta, mean, rstd, groups, act=None, slope=0.2):
+    """-> dx like x, dgamma, dbeta (C,) fp32."""
+    B, N, C, groups, dt = sizes = _gn_sizes(x, gamma, beta, groups, act)
+    _chk(dy, x.dtype, "dy"); _chk(mean, F32, "mean"); _chk(rstd, F32, "rstd")
+    _chk_device("group_norm", dy, mean, rstd)
+    if dy.shape != x.shape or tuple(mean.shape) != (B, groups) or tuple(rstd.shape) != (B, groups):
+        raise RuntimeError("group_norm: dy, mean or rstd does not match x")
+    dx = torch.empty_like(x)
+    grads = torch.empty(2, C, dtype=F32, device=x.device)
+    ws = _gn_workspace(sizes, True, x.device)
+    rc = _timed("gn_bwd", 0, 3 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_bwd(
+        _ptr(x), _ptr(dy), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(grads[0]), _ptr(grads[1]), _ptr(ws),
+        B, N, C, groups, dt, ACTS[act], float(slope), _stream()))
+    _lib.check(rc, "rgbd_group_norm_bwd")
+    return dx, grads[0], grads[1]
+
+
+class _AttnDesc(ctypes.Structure):          # rgbd_attn_desc (include/rgbd_gan_hip.h)
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")]
+                + [(f"{t}_s{a}", ctypes.c_int64) for t in "qkv" for a in "blh"]
+                + [(n, ctypes.c_void_p) for n in ("table", "map", "lengths", "lse")]
+                + [(n, ctypes.c_int) for n in ("B", "H", "Hkv", "Lq", "Lk", "D", "rows", "cols", "q_start", "n_buckets")]
+                + [(n, ctypes.c_float) for n in ("scale", "cap")] + [("fine", ctypes.c_int)])
+
+
+class _AttnGrad(ctypes.Structure):          # rgbd_attn_grad
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("d_o", "o", "o_lo", "dq", "dk", "dv")]
+                + [(f"{t}_s{a}", ctypes.c_int64) for t in ("dq", "dk", "dv") for a in "blh"]
+                + [(n, ctypes.c_void_p) for n in ("dtable", "order", "start")])
+
+
+HEAD_SIZES = (32, 64, 128)
+
+
+def attention_readable(t):
+    """Can the kernels read `t` (B, L, heads, D) as it lies: contiguous head vectors, 16-byte aligned."""
+    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t))
+
+
+def _strides(t):
+    """Strides of the first three axes; an axis of one (or no) element has none that matters."""
+    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]
+
+
+def _attn_desc(q, k, v, table, buckets, lengths, scale, cap, q_start):
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if not torch.is_tensor(t) or t.dim() != 4:
+            raise RuntimeError(f"attention: {name} must be (B, tokens, heads, head size)")
+        if t.dtype != BF16:
+            raise RuntimeError(f"attention: {name} must be bf16, got {t.dtype}")
+    B, Lq, H, D = q.shape
+    if D not in HEAD_SIZES:
+        raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
+    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+        raise RuntimeError(f"attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+    Lk, Hkv = k.shape[1], k.shape[2]
+    if H < 1 or Hkv < 1 or H % Hkv:
+        raise RuntimeError(f"attention: {Hkv} key / value heads do not divide {H} query heads")
+    if not cap >= 0:
+        raise RuntimeError(f"attention: cap must not be negative, got {cap}")
+    if (table is None) != (buckets is None):
+        raise RuntimeError("attention: a bias table and its buckets come together")
+    rows = cols = n_buckets = 0
+    if table is not None:
+        rows, cols, n_buckets = buckets.rows, buckets.cols, buckets.n_buckets
+        if tuple(table.shape) != (H, n_buckets):
+            raise RuntimeError(f"attention: table must be ({H}, {n_buckets}), got {tuple(table.shape)}")
+        if rows > 1 and cols > 1024:
+            raise RuntimeError(f"attention: a grid of more than one row has at most 1024 columns, got {cols}")
+        if q_start < 0 or q_start + Lq > rows * cols or Lk > rows * cols:
+            raise RuntimeError(f"attention: tokens outside the {rows} x {cols} grid (q_start {q_start}, {Lq} queries, {Lk} keys)")
+    elif q_start:
+        raise RuntimeError("attention: q_start places the queries on the bias's grid: it needs a table")
+    if lengths is not None and tuple(lengths.shape) != (B,):
+        raise RuntimeError(f"attention: lengths must be ({B},), got {tuple(lengths.shape)}")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if not t.is_cuda:
+            raise RuntimeError(f"{name}: expected a GPU tensor (the HIP path has no CPU fallback)")
+        if not attention_readable(t):
+            raise RuntimeError(f"attention: {name}: head vectors must be contiguous, strides multiples of 8, 16-byte aligned")
+    _chk(table, F32, "table"); _chk(lengths, torch.int32, "lengths")
+    _chk_device("attention", q, k, v, table, lengths, buckets.map if buckets is not None else None)
+    d = _AttnDesc()
+    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    d.q_sb, d.q_sl, d.q_sh = _strides(q)
+    d.k_sb, d.k_sl, d.k_sh = _strides(k)
+    d.v_sb, d.v_sl, d.v_sh = _strides(v)
+    if table is not None:
+        d.table, d.map = table.data_ptr(), buckets.map.data_ptr()
+    if lengths is not None:
+        d.lengths = lengths.data_ptr()
+    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D = B, H, Hkv, Lq, Lk, D
+    d.rows, d.cols, d.q_start, d.n_buckets = rows, cols, q_start, n_buckets
+    d.scale, d.cap = scale, cap
+    return d
+
+
+def attention_fwd(q, k, v, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, keep=False, fine=False):
+    """q (B, Lq, H, D), k, v (B, Lk, Hkv, D) bf16 (attention_readable) -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward
+    pass needs: o_lo (what rounding o dropped, bf16) and lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient
+    needs of o (probabilities with 16 bits in the second product)."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    d = _attn_desc(q, k, v, table, buckets, lengths, scale, float(cap or 0.0), int(q_start))
+    o = torch.empty(d.B, d.Lq, d.H, d.D, dtype=BF16, device=q.device)
+    o_lo = lse = None
+    d.fine = int(fine)
+    if keep:
+        o_lo = torch.empty_like(o)
+        lse = torch.empty(d.B, d.H, d.Lq, dtype=F32, device=q.device)
+        d.lse = lse.data_ptr()
+    flops = 4 * d.B * d.H * d.Lq * d.Lk * d.D
+    rc = _timed("attn_fwd", flops, 4 * o.numel() + 4 * k.numel(), lambda: _lib.load().rgbd_attention_fwd(
+        ctypes.byref(d), _ptr(o), _ptr(o_lo), _stream()))
+    _lib.check(rc, "rgbd_attention_fwd")
+    return o, o_lo, lse
+
+
+def attention_bwd(q, k, v, d_o, o, o_lo, lse, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, out=None,
+                  want_table=True):
+    """-> dq, dk, dv (views of `out` = three (B, L, heads, D) bf16 tensors where given), dtable (None unless wanted)."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    d = _attn_desc(q, k, v, table, buckets, lengths, scale, float(cap or 0.0), int(q_start))
+    for t, name in ((d_o, "d_o"), (o, "o"), (o_lo, "o_lo")):
+        _chk(t, BF16, name)
+        if t.shape != q.shape:
+            raise RuntimeError(f"attention: {name} {tuple(t.shape)} does not match q {tuple(q.shape)}")
+    _chk(lse, F32, "lse")
+    if tuple(lse.shape) != (d.B, d.H, d.Lq):
+        raise RuntimeError(f"attention: lse must be {(d.B, d.H, d.Lq)}, got {tuple(lse.shape)}")
+    _chk_device("attention", d_o, o, o_lo, lse)
+    d.lse = lse.data_ptr()
+    if out is None:
+        out = tuple(torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
+    for t, ref in zip(out, (q, k, v)):
+        if t.dtype != BF16 or t.shape != ref.shape or not attention_readable(t) or t.device != q.device:
+            raise RuntimeError("attention: a gradient buffer does not match its tensor")
+    want_table = bool(want_table and table is not None)
+    dtable = torch.empty_like(table) if want_table else None
+    g = _AttnGrad()
+    g.d_o, g.o, g.o_lo = d_o.data_ptr(), o.data_ptr(), o_lo.data_ptr()
+    g.dq, g.dk, g.dv = (t.data_ptr() for t in out)
+    g.dq_sb, g.dq_sl, g.dq_sh = _strides(out[0])
+    g.dk_sb, g.dk_sl, g.dk_sh = _strides(out[1])
+    g.dv_sb, g.dv_sl, g.dv_sh = _strides(out[2])
+    if want_table:
+        g.dtable, g.order, g.start = dtable.data_ptr(), buckets.order.data_ptr(), buckets.start.data_ptr()
+    lib = _lib.load()
+    n = lib.rgbd_attention_bwd_workspace(ctypes.byref(d), int(want_table))
+    if n < 0:
+        _lib.check(-1, "rgbd_attention_bwd_workspace")
+    ws = torch.empty(n, dtype=F32, device=q.device)
+    flops = 10 * d.B * d.H * d.Lq * d.Lk * d.D
+    rc = _timed("attn_bwd", flops, 8 * q.numel() + 8 * k.numel(), lambda: lib.rgbd_attention_bwd(
+        ctypes.byref(d), ctypes.byref(g), _ptr(ws), _stream()))
+    _lib.check(rc, "rgbd_attention_bwd")
+    return (*out, dtable)
