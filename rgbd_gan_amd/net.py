@@ -64,6 +64,17 @@ def _synthesis_chans(ch, nb):
     return [(ch, ch)] * 4 + [(ch >> (i - 3), ch >> (i - 4)) for i in range(4, nb)]
 
 
+def attention_sizes(value, nb):
+    """The `self_attention` option -> sorted map sizes: None / 0, a size, a list of sizes or "16,32"; sizes of the nb blocks."""
+    if isinstance(value, str):
+        value = [v for v in value.replace(",", " ").split()]
+    sizes = sorted({int(v) for v in (value if isinstance(value, (list, tuple)) else [value or 0])} - {0})
+    for s in sizes:
+        if s not in [4 << i for i in range(nb)]:
+            raise ValueError(f"self_attention: {s} is not the size of a block ({', '.join(str(4 << i) for i in range(nb))})")
+    return sizes
+
+
 def _split_stage(stage, max_stage):
     stage = min(stage, max_stage - 1e-8)
     fl = math.floor(stage)
@@ -153,12 +164,40 @@ class MappingNetwork(_Link):
     forward = __call__
 
 
+class SelfAttention:
+    """h + out(attention(qkv(group_norm(h)))) over the pixels of an (B, size, size, C) feature map: heads of 64 channels, a learned
+    bias by relative position (15 logarithmic buckets an axis), scores capped at 50.  Not a reference layer: an option of this
+    engine's generator (`self_attention`).  `out` starts at zero, so a new layer is the identity."""
+
+    HEAD, BUCKETS, CAP = 64, 15, 50.0
+
+    @classmethod
+    def specs(cls, pre, c):
+        return [(pre + "/norm/gamma", (c,), "ones"), (pre + "/norm/beta", (c,), "zeros"),
+                (pre + "/qkv/c/W", (3 * c, c, 1, 1), "normal"), (pre + "/table", (c // cls.HEAD, cls.BUCKETS ** 2), "zeros"),
+                (pre + "/out/c/W", (c, c, 1, 1), "zeros"), (pre + "/out/c/b", (c,), "zeros")]
+
+    def __init__(self, params, pre, c, size, device):
+        self.p, self.pre, self.c = params, pre, c
+        self.buckets = Fn.RelativeBuckets.log(size, size, self.BUCKETS, size, device=device)
+        self.qkv = Fn.ConvLayer(params[pre + "/qkv/c/W"], _inv_c(c, 1.0), 0)
+        self.out = Fn.ConvLayer(params[pre + "/out/c/W"], _inv_c(c, 1.0), 0)
+
+    def __call__(self, h):
+        p, pre = self.p, self.pre
+        x = Fn.group_norm(h, p[pre + "/norm/gamma"], p[pre + "/norm/beta"], 32)
+        o = Fn.attention_packed(Fn.conv(x, self.qkv), self.c // self.HEAD, table=p[pre + "/table"], buckets=self.buckets, cap=self.CAP)
+        return Fn.conv_bias(o.reshape(h.shape), self.out, p[pre + "/out/c/b"], residual=h)
+
+
 class StyleGenerator(_Link):
     """net.py:164-311.  Channel plan at ch: blocks (ch,ch,ch,ch,ch/2,ch/4) at 4..128 px; max_resolution 256 / 512 adds
-    the blocks the reference keeps commented out (ch/8 at 256 px, ch/16 at 512 px: net.py:181-183,192-194)."""
+    the blocks the reference keeps commented out (ch/8 at 256 px, ch/16 at 512 px: net.py:181-183,192-194).
+    self_attention (not a reference argument): map sizes whose block is followed by a SelfAttention layer."""
 
-    def __init__(self, ch, device, rgbd=True, initial_depth=1.0, seed=1, enable_blur=False, max_resolution=128):
+    def __init__(self, ch, device, rgbd=True, initial_depth=1.0, seed=1, enable_blur=False, max_resolution=128, self_attention=None):
         nb = _block_count(max_resolution)
+        attend = attention_sizes(self_attention, nb)
         self.ch, self.rgbd, self.max_stage = ch, rgbd, 2 * nb + 5     # 17 for the reference's six blocks (net.py:166)
         self.enable_blur = bool(enable_blur)       # net.py:140-141: c0(blur(upscale2x(h))) instead of c0(upscale2x(h))
         self.chans = _synthesis_chans(ch, nb)      # (out, in)
@@ -187,13 +226,18 @@ class StyleGenerator(_Link):
         if rgbd:
             specs += [("l1/c/W", (ch, ch + 9), "normal"), ("l1/c/b", (ch,), "zeros"),
                       ("l2/c/W", (ch, ch), "normal"), ("l2/c/b", (ch,), "zeros")]
+        for size in attend:
+            i = size.bit_length() - 3
+            specs += SelfAttention.specs(f"attention/{i}", self.chans[i][0])
         self.store = ParamStore(specs, device, seed)
         self.stores = (("", self.store),)
         p = self.store.params
+        self.attention = {size.bit_length() - 3: SelfAttention(p, f"attention/{size.bit_length() - 3}",
+                                                               self.chans[size.bit_length() - 3][0], size, device) for size in attend}
         self.c0 = [None] + [Fn.ConvLayer(p[f"blocks/{i}/c0/c/W"], _inv_c(self.chans[i][1] * 9), 1)
                             for i in range(1, nb)]
         self.c1 = [Fn.ConvLayer(p[f"blocks/{i}/c1/c/W"], _inv_c(self.chans[i][0] * 9), 1) for i in range(nb)]
-        self.pack_group = Fn.PackGroup(self.c0 + self.c1)
+        self.pack_group = Fn.PackGroup(self.c0 + self.c1 + [c for a in self.attention.values() for c in (a.qkv, a.out)])
 
     # -- pieces
     def _style(self, name, w, h):
@@ -222,6 +266,10 @@ class StyleGenerator(_Link):
         return {k: (group, j) for j, k in enumerate(keys)}
 
     def _block(self, i, w, x, styles=None):
+        h = self._synthesis(i, w, x, styles)
+        return self.attention[i](h) if i in self.attention else h
+
+    def _synthesis(self, i, w, x, styles=None):
         """net.py:130-161 (SynthesisBlock.forward), add_noise False (forced at net.py:243).  `styles`: the windows of
         a _style_group covering this block (else its two affines are computed here from `w`)."""
         p = self.store.params
@@ -312,9 +360,11 @@ class StyleGenerator(_Link):
 
 class StyleGANGenerator(_Link):
     def __init__(self, ch, enable_blur=False, rgbd=False, rotate_conv_input=False, use_encoder=False,
-                 use_occupancy_net=False, initial_depth=None, device="cuda:0", seed=0, max_resolution=128):
+                 use_occupancy_net=False, initial_depth=None, device="cuda:0", seed=0, max_resolution=128,
+                 self_attention=None):
         """max_resolution (not a reference argument: its 256+ blocks are commented out in the source, net.py:181-183): 256
-        needs ch = 512 (ch/8 = 64 channels in the last block)."""
+        needs ch = 512 (ch/8 = 64 channels in the last block).  self_attention (not a reference argument either): the map sizes
+        (32, [16, 32] or "16,32") whose block is followed by a SelfAttention layer."""
         assert not rotate_conv_input and not use_encoder and not use_occupancy_net, "unsupported generator option"
         assert ch % 256 == 0, "the MFMA conv engine needs ch/4 to be a multiple of 64"
         self.ch = ch
@@ -322,7 +372,7 @@ class StyleGANGenerator(_Link):
         self.device = torch.device(device)
         self.mapping = MappingNetwork(ch, device, seed)
         self.gen = StyleGenerator(ch, device, rgbd, 1.0 if initial_depth is None else initial_depth, seed + 1,
-                                  enable_blur=bool(enable_blur), max_resolution=max_resolution)
+                                  enable_blur=bool(enable_blur), max_resolution=max_resolution, self_attention=self_attention)
         self.stores = (("mapping/", self.mapping.store), ("gen/", self.gen.store))
         self.train = True
 

@@ -18,7 +18,10 @@ def setup_generator(config, device, seed=0):
         return StyleGANGenerator(config.ch, enable_blur=config.enable_blur, rgbd=rgbd,
                                  rotate_conv_input=config.rotate_conv_input, use_encoder=config.bigan,
                                  use_occupancy_net=config.use_occupancy_net_loss, initial_depth=config.initial_depth,
-                                 device=device, seed=seed, max_resolution=config.max_resolution or 128)
+                                 device=device, seed=seed, max_resolution=config.max_resolution or 128,
+                                 self_attention=config.self_attention)      # optional YAML key of this engine
+    if config.self_attention:
+        raise AssertionError(f"self_attention is an option of the stylegan generator, not of {arch}")
     if arch == "dcgan":
         # NB the reference passes config.ch as in_ch and leaves ch at its default 512 (train_rgbd.py:230)
         return DCGANGenerator(config.ch, enable_blur=config.enable_blur, rgbd=rgbd, use_encoder=config.bigan,

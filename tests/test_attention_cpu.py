@@ -175,3 +175,18 @@ def test_oracle_group_norm_gradients_match_differences(act):
     g = torch.Generator().manual_seed(0)
     r = lambda *s: torch.randn(*s, generator=g, dtype=F64).requires_grad_(True)
     assert torch.autograd.gradcheck(lambda x, a, b: ref.group_norm(x, a, b, 2, act=act), (r(2, 3, 2, 6), r(6), r(6)), eps=1e-6, atol=1e-6)
+
+
+# ------------------------------------------------------------------------------------------------ the generator's option
+def test_self_attention_option():
+    from rgbd_gan_amd.net import attention_sizes
+    from rgbd_gan_amd.training import setup_generator
+    from rgbd_gan_amd.utils.yaml_utils import Config
+    for value, want in ((None, []), (0, []), (32, [32]), ([32, 16], [16, 32]), ("16, 32", [16, 32]), ("64", [64]), ("", [])):
+        assert attention_sizes(value, 6) == want
+    for bad in (24, 256, [16, 5], "2"):
+        with pytest.raises(ValueError):
+            attention_sizes(bad, 6)
+    for arch in ("dcgan", "deepvoxels"):
+        with pytest.raises(AssertionError, match="self_attention"):
+            setup_generator(Config(dict(generator_architecture=arch, ch=256, self_attention=32)), "cpu")
