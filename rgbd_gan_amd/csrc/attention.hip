@@ -34,7 +34,7 @@ struct AttnArgs {
     int64_t dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
     int B, H, Hkv, rep, Lq, Lk;
     int rows, cols, q_start, n_buckets;
-    int n_qb, n_kb, seg_tiles;
+    int n_qb, n_kb, n_kt, seg_tiles;
     int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
     float scale, cap;
 };
@@ -110,6 +110,13 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int i0) {
 }
 __device__ __forceinline__ float other_half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float other_half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
+
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+// LDS operations of one wave complete in order; this keeps the compiler to that order where lanes read what others wrote
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // tanh of 16 values.  Below 0.5 an odd polynomial (least squares on Chebyshev nodes, relative error 1.1e-7: there the quotient
 // form would lose digits by cancellation, and capped scores mostly lie there); beyond it 1 - 2 / (e^2x + 1).
@@ -356,12 +363,23 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
 }
 
 // ======================================================================================================= dq, delta and the table
-// Partials of the table's gradient: a pair of tokens (i, j) is known by its distance i - j and by whether the column of i wraps
-// (class 0: dx >= 0, class 1: dx < 0): the two together are the offset.  ds goes through LDS in fp32 and a thread adds up one
-// diagonal of the tile; a diagonal stays with its thread (distance mod 256) over the three tiles it crosses and is then stored
-// once, so no atomics, no clearing and one order of summation.
-// LDS: K[2] V[2] | at[2][64] | ds (64 x 128 fp32, where the table's gradient is wanted) | window.
-template <int D, int BIAS, bool CAP, bool DT>
+// Partials of the table's gradient, without global atomics and in one order of summation.  DT names how a 128 x 64 tile of ds (fp32,
+// never rounded) is reduced to sums over pairs of equal offset:
+//   BLOCKS    where 32 aligned tokens lie in one row of the grid (columns a multiple of 32, or a single row): within a 32 x 32 block
+//             the offset is one number plus (query - key), 63 sums.  A wave puts its block into LDS of its own (no barrier), rows
+//             of 32 values and 40 zeros: a lane then adds up one diagonal, 32 reads at fixed distances that run off the block into
+//             zeros, no comparison.  part (b, h, query group, key group, 64).  (Adding with ds_add_f32 instead took 2.8 times the
+//             whole kernel's time: 728 us against 264 with diagonals at 32 samples x 4 heads x 1024 tokens.)
+//   DIAGONALS any other grid: a pair is known by its distance i - j and by whether the column of i wraps (class 0: dx >= 0, class 1:
+//             dx < 0).  ds goes through LDS and a thread adds up one diagonal of the tile; a diagonal stays with its thread (distance
+//             mod 256) over the three tiles it crosses and is stored once: part (b, h, query block, class, distance).
+// LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (64 x 128 floats) | window.
+enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
+constexpr int BS = 72;                    // floats from row to row of a block: rows 4 apart (a wave's halves) are 32 banks apart
+constexpr int BLOCK_FLOATS = 32 + 32 * BS;
+constexpr int DT_LDS[3] = {0, 4 * BLOCK_FLOATS * 4, KT * BLK * 4};
+
+template <int D, int BIAS, bool CAP, int DT>
 __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
@@ -369,7 +387,8 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     char* vt = smem + 2 * TB;
     int* at = reinterpret_cast<int*>(smem + 4 * TB);
     float* dsl = reinterpret_cast<float*>(smem + 4 * TB + 2 * KT * 4);
-    float* win = dsl + (DT ? KT * BLK : 0);
+    float* win = dsl + DT_LDS[DT] / 4;
+    const int n_kg = a.n_kt * 2;
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
     const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
@@ -377,6 +396,11 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     const int row = qb * BLK + wave * 32 + (lane & 31);
     const bool live = row < a.Lq;
     const Frags<D> fr(lane);
+    float* blk = dsl + wave_id() * BLOCK_FLOATS + 32;                // BLOCKS: row 0, zeros in front of it
+    if (DT == DT_BLOCKS) {
+        for (int i = lane; i < BLOCK_FLOATS; i += 64) blk[i - 32] = 0.f;
+        wave_fence();
+    }
 
     bf16x8 qf[KS], gf[KS];
     float delta = 0.f;
@@ -413,8 +437,9 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
     float sum0 = 0.f, sum1 = 0.f;                                    // the thread's diagonal, by class
-    // partials of this workgroup, place 0 = the smallest distance it meets
-    float* part = DT ? a.part + (int64_t)id * 2 * a.span : nullptr;
+    // DIAGONALS: partials of this workgroup, place 0 = the smallest distance it meets
+    float* part = DT == DT_DIAGONALS ? a.part + (int64_t)id * 2 * a.span
+                                     : DT == DT_BLOCKS ? a.part + ((int64_t)id * 4 + wave) * n_kg * 64 : nullptr;
     const int d_min = tq0 - (nt * KT - 1);
 
     Stage<D> sk, sv;
@@ -463,8 +488,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float ds = __builtin_amdgcn_exp2f(s[i] - lse) * (dp[i] - delta);
-                if (DT) dsl[(32 * u + 8 * (i >> 2) + 4 * half + (i & 3)) * BLK + wave * 32 + (lane & 31)] = ds;
+                if (DT == DT_DIAGONALS) dsl[(32 * u + 8 * (i >> 2) + 4 * half + (i & 3)) * BLK + wave * 32 + (lane & 31)] = ds;
+                if (DT == DT_BLOCKS) blk[(8 * (i >> 2) + 4 * half + (i & 3)) * BS + (lane & 31)] = ds;
                 s[i] = CAP ? ds * (1.f - th[i] * th[i]) : ds;
+            }
+            if (DT == DT_BLOCKS) {                                   // lane: query - key = lane - 32
+                wave_fence();
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 32; ++i) sum += blk[i * (BS + 1) + lane - 32];
+                part[(2 * t + u) * 64 + lane] = sum;
+                wave_fence();
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
@@ -478,7 +512,7 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             sv.store(vt + ((t + 1) & 1) * TB);
             places(t + 1);
         }
-        if (DT) {
+        if (DT == DT_DIAGONALS) {
             __syncthreads();
             const int k0 = t * KT, lo = tq0 - k0 - (KT - 1);         // smallest distance of this tile
             const int w = ((int)threadIdx.x - lo) & 255;
@@ -486,19 +520,20 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
             if (c < BLK) {
                 const int k_lo = max(0, -c), k_hi = min(KT - 1, BLK - 1 - c);
                 const float* p = dsl + k_lo * (BLK + 1) + c;
-                if (a.rows == 1) {
-                    for (int k = k_lo; k <= k_hi; ++k, p += BLK + 1) sum0 += *p;
-                } else {
-                    int r = dist % a.cols;
-                    r += r < 0 ? a.cols : 0;
-                    int x = (k0 + k_lo) % a.cols + r - a.cols;       // >= 0: the column of i wraps
-                    const int wrap = r;
-                    for (int k = k_lo; k <= k_hi; ++k, p += BLK + 1) {
-                        const float v = *p;
-                        if (x >= 0) sum1 += v;
-                        else sum0 += v;
+                int r = dist % a.cols;
+                r += r < 0 ? a.cols : 0;
+                int x = (k0 + k_lo) % a.cols + r - a.cols;           // >= 0: the column of i wraps
+                for (int k = k_lo; k <= k_hi; k += 8, p += 8 * (BLK + 1)) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = k + j <= k_hi ? p[j * (BLK + 1)] : 0.f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float w = x >= 0 ? v[j] : 0.f;
+                        sum1 += w;
+                        sum0 += v[j] - w;
                         ++x;
-                        if (x == wrap) x -= a.cols;                  // the key's own row ends
+                        x -= x == r ? a.cols : 0;                    // the key's own row ends
                     }
                 }
                 if (c >= KT || t + 1 == nt) {                        // the diagonal leaves the workgroup's rows
@@ -521,40 +556,94 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
         }
 }
 
-// ---- the table's gradient from the partials: by distance and class first, then by bucket.
-// by_dist (H, 2, 2 n - 1): grid (distances / 256, 2 classes x H); a thread adds its distance over samples and query blocks.
-__global__ __launch_bounds__(256) void attn_dist_kernel(AttnArgs a, float* by_dist, int n_dist, int d0) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    const int cls = blockIdx.y & 1, h = blockIdx.y >> 1;
-    if (i >= n_dist) return;
-    const int dist = i + d0;
+// ---- the table's gradient from the partials: sums over samples and places first, then by bucket.
+// BLOCKS.  by_block (H, classes, 64): a class is (row difference, column-group difference) of a block's query and key groups, G =
+// columns / 32 groups a row (a single row: G = all of them).  grid (classes, H), 16 row lanes x 64 places.
+__global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float* by_block, int q_row0, int q_rows, int k_rows, int gq, int gk) {
+    __shared__ float red[1024];
+    const int cls = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, r = threadIdx.x >> 6;
+    const int dgs = gq + gk - 1;
+    const int dy = cls / dgs - (k_rows - 1), dg = cls % dgs - (gk - 1);       // query group row (from q_row0) - key row, group - group
+    const int y0 = max(0, dy), y1 = min(q_rows, k_rows + dy), g0 = max(0, dg), g1 = min(gq, gk + dg);
+    const int ny = max(0, y1 - y0), ng = max(0, g1 - g0), n = a.B * ny * ng;
+    const int n_qg = a.n_qb * 4, n_kg = a.n_kt * 2;
     float s = 0.f;
-    for (int b = 0; b < a.B; ++b) {
-        const int nt = (keys_of(a, b) + KT - 1) / KT;
-        if (nt == 0) continue;
-        for (int qb = 0; qb < a.n_qb; ++qb) {
-            const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * KT - 1));
-            if (place < 0 || dist > tq0 + BLK - 1) continue;
-            s += a.part[((int64_t)((b * a.H + h) * a.n_qb + qb) * 2 + cls) * a.span + place];
-        }
+    for (int e = r; e < n; e += 16) {
+        const int g = g0 + e % ng, y = y0 + e / ng % ny, b = e / (ng * ny);
+        const int qg = y * gq + g, kg = (y - dy) * gk + g - dg;
+        if (qg >= n_qg || kg >= 2 * ((keys_of(a, b) + KT - 1) / KT)) continue;
+        s += a.part[((int64_t)((b * a.H + h) * n_qg + qg) * n_kg + kg) * 64 + lane];
     }
-    by_dist[((int64_t)h * 2 + cls) * n_dist + i] = s;
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (r == 0) {
+        for (int k = 1; k < 16; ++k) s += red[k * 64 + lane];
+        by_block[((int64_t)h * gridDim.x + cls) * 64 + lane] = s;
+    }
 }
 
-// dtable[h][u] = sum over the offsets of bucket u (order[start[u]] .. ): grid (n_buckets, H), a wave each.
-__global__ __launch_bounds__(64) void attn_bucket_kernel(AttnArgs a, const float* by_dist, const int* order, const int* start, int n_dist,
-                                                         int d0) {
+// dtable[h][u] = sum over the offsets of bucket u (order[start[u]] .. ): grid (n_buckets, H).  An offset lies in two neighbouring
+// classes of blocks.
+__global__ __launch_bounds__(256) void attn_block_bucket_kernel(AttnArgs a, const float* by_block, const int* order, const int* start, int q_row0,
+                                                                int k_rows, int q_rows, int gq, int gk) {
+    __shared__ float red[4];
+    const int u = blockIdx.x, h = blockIdx.y, w = 2 * a.cols - 1, dgs = gq + gk - 1;
+    const float* src = by_block + (int64_t)h * (q_rows + k_rows - 1) * dgs * 64;
+    float s = 0.f;
+    for (int e = start[u] + (int)threadIdx.x; e < start[u + 1]; e += 256) {
+        const int off = order[e];
+        int dy = off / w - (a.rows - 1), dx = off % w - (a.cols - 1);
+        if (a.rows == 1) dx -= a.q_start;                              // groups count from the first query
+        dy -= q_row0;
+        if (dy < -(k_rows - 1) || dy > q_rows - 1) continue;
+        const int lo = dx >> 5, c = dx & 31;                           // dx = 32 lo + c = 32 (lo + 1) - (32 - c)
+        const float* row = src + (int64_t)(dy + k_rows - 1) * dgs * 64;
+        const int g = lo + gk - 1;
+        if (g >= 0 && g < dgs) s += row[g * 64 + 32 + c];
+        if (c && g + 1 >= 0 && g + 1 < dgs) s += row[(g + 1) * 64 + c];
+    }
+    s = wave_sum(s);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.dtable[(int64_t)h * a.n_buckets + u] = red[0] + red[1] + red[2] + red[3];
+}
+
+// DIAGONALS.  by_dist (H, 2, n_dist): grid (distances / 64, 2 classes x H), 16 row lanes x 64 distances.
+__global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_dist, int n_dist, int d0) {
+    __shared__ float red[1024];
+    const int i = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+    const int cls = blockIdx.y & 1, h = blockIdx.y >> 1, dist = i + d0;
+    float s = 0.f;
+    for (int e = r; e < a.B * a.n_qb; e += 16) {
+        const int qb = e % a.n_qb, b = e / a.n_qb;
+        const int nt = (keys_of(a, b) + KT - 1) / KT;
+        const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * KT - 1));
+        if (nt == 0 || place < 0 || dist > tq0 + BLK - 1) continue;
+        s += a.part[((int64_t)((b * a.H + h) * a.n_qb + qb) * 2 + cls) * a.span + place];
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (r == 0 && i < n_dist) {
+        for (int k = 1; k < 16; ++k) s += red[k * 64 + (threadIdx.x & 63)];
+        by_dist[((int64_t)h * 2 + cls) * n_dist + i] = s;
+    }
+}
+
+__global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const float* by_dist, const int* order, const int* start, int n_dist,
+                                                               int d0) {
+    __shared__ float red[4];
     const int u = blockIdx.x, h = blockIdx.y, w = 2 * a.cols - 1;
     const float* src = by_dist + (int64_t)h * 2 * n_dist;
     float s = 0.f;
-    for (int e = start[u] + (int)threadIdx.x; e < start[u + 1]; e += 64) {
+    for (int e = start[u] + (int)threadIdx.x; e < start[u + 1]; e += 256) {
         const int off = order[e], dy = off / w - (a.rows - 1), dx = off % w - (a.cols - 1);
         const int place = dy * a.cols + dx - d0;
-        const int cls = a.rows > 1 && dx < 0 ? 1 : 0;
-        if (place >= 0 && place < n_dist) s += src[(int64_t)cls * n_dist + place];
+        if (place >= 0 && place < n_dist) s += src[(int64_t)(dx < 0) * n_dist + place];
     }
     s = wave_sum(s);
-    if (threadIdx.x == 0) a.dtable[(int64_t)h * a.n_buckets + u] = s;
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) a.dtable[(int64_t)h * a.n_buckets + u] = red[0] + red[1] + red[2] + red[3];
 }
 
 // ======================================================================================================= dk, dv
@@ -705,13 +794,13 @@ int span_of(int n, int rows, int cols) {                              // the mos
     const int64_t s = (n - 1) + crossings * (cols - 1);
     return s > (1 << 30) ? 1 << 30 : (int)s;
 }
-int segment_tiles(int owned, int streamed, int rows, int cols) {
+int segment_tiles(int owned, int streamed, int rows, int cols, int floats = WIN_FLOATS) {
     const int own = span_of(owned < BLK ? owned : BLK, rows, cols);
     const int tiles = ceil_div(streamed, KT);
     int lo = 0;
     for (int t = tiles; t > 0; t = t > 64 ? t / 2 : t - 1) {
         const int64_t n = (int64_t)t * KT < streamed ? (int64_t)t * KT : streamed;
-        if ((int64_t)own + span_of((int)n, rows, cols) + 1 <= WIN_FLOATS) { lo = t; break; }
+        if ((int64_t)own + span_of((int)n, rows, cols) + 1 <= floats) { lo = t; break; }
     }
     return lo;
 }
@@ -752,7 +841,7 @@ AttnArgs args_of(const rgbd_attn_desc* d) {
     a.rows = d->table ? d->rows : 1; a.cols = d->table ? d->cols : 1 << 24; a.q_start = d->table ? d->q_start : 0;
     a.n_buckets = d->n_buckets;
     a.scale = d->scale; a.cap = d->cap;
-    a.n_qb = ceil_div(d->Lq, BLK); a.n_kb = ceil_div(d->Lk, BLK);
+    a.n_qb = ceil_div(d->Lq, BLK); a.n_kb = ceil_div(d->Lk, BLK); a.n_kt = ceil_div(d->Lk, KT);
     a.lse = d->lse;
     return a;
 }
@@ -787,10 +876,15 @@ template <int D> int launch_fwd(const AttnArgs& a, int bias, bool cap, bool fine
     else { if (bias == 1) LAUNCH((attn_fwd_kernel<D, 1, false, true>)); else LAUNCH((attn_fwd_kernel<D, 2, false, true>)); }
     return 0;
 }
-template <int D> int launch_dq(const AttnArgs& a, int bias, bool cap, bool dt, unsigned grid, size_t lds, hipStream_t s) {
-    if (!dt) { BY_BIAS_CAP(attn_dq_kernel, D, , false); return 0; }
-    if (cap) { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, true, true>)); else LAUNCH((attn_dq_kernel<D, 2, true, true>)); }
-    else { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, false, true>)); else LAUNCH((attn_dq_kernel<D, 2, false, true>)); }
+template <int D> int launch_dq(const AttnArgs& a, int bias, bool cap, int dt, unsigned grid, size_t lds, hipStream_t s) {
+    if (dt == DT_NONE) { BY_BIAS_CAP(attn_dq_kernel, D, , DT_NONE); return 0; }
+    if (dt == DT_BLOCKS) {                                            // 32 aligned tokens in a row: four are too
+        if (cap) LAUNCH((attn_dq_kernel<D, 2, true, DT_BLOCKS>));
+        else LAUNCH((attn_dq_kernel<D, 2, false, DT_BLOCKS>));
+        return 0;
+    }
+    if (cap) { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, true, DT_DIAGONALS>)); else LAUNCH((attn_dq_kernel<D, 2, true, DT_DIAGONALS>)); }
+    else { if (bias == 1) LAUNCH((attn_dq_kernel<D, 1, false, DT_DIAGONALS>)); else LAUNCH((attn_dq_kernel<D, 2, false, DT_DIAGONALS>)); }
     return 0;
 }
 template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned grid, size_t lds, hipStream_t s) {
@@ -798,17 +892,29 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
     return 0;
 }
 
-struct BwdSizes { int64_t delta, part, by_dist; int span, n_dist, d0; };
+// Floats of the backward workspace: delta, the partials and what the first reduction leaves of them.
+struct BwdSizes { int64_t delta, part, sums; int mode, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
 BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};
     z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
-    if (dt && d->Lq > 0 && d->Lk > 0) {
-        const int n_qb = ceil_div(d->Lq, BLK);
-        z.span = ceil_div(d->Lk, KT) * KT + BLK;
+    if (!dt || d->Lq == 0 || d->Lk == 0) return z;
+    const int n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
+    if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
+        z.mode = DT_BLOCKS;
+        z.part = (int64_t)d->B * d->H * n_qb * 4 * n_kt * 2 * 64;
+        z.gq = d->rows == 1 ? n_qb * 4 : d->cols / 32;
+        z.gk = d->rows == 1 ? n_kt * 2 : d->cols / 32;
+        z.q_row0 = d->rows == 1 ? 0 : d->q_start / d->cols;
+        z.q_rows = d->rows == 1 ? 1 : ceil_div(d->Lq, d->cols);
+        z.k_rows = d->rows == 1 ? 1 : ceil_div(d->Lk, d->cols);
+        z.sums = (int64_t)d->H * (z.q_rows + z.k_rows - 1) * (z.gq + z.gk - 1) * 64;
+    } else {
+        z.mode = DT_DIAGONALS;
+        z.span = n_kt * KT + BLK;
         z.part = (int64_t)d->B * d->H * n_qb * 2 * z.span;
-        z.d0 = d->q_start - (ceil_div(d->Lk, KT) * KT - 1);           // distances from there to q_start + n_qb * BLK - 1
+        z.d0 = d->q_start - (n_kt * KT - 1);                          // distances from there to q_start + n_qb * BLK - 1
         z.n_dist = d->q_start + n_qb * BLK - z.d0;
-        z.by_dist = (int64_t)d->H * 2 * z.n_dist;
+        z.sums = (int64_t)d->H * 2 * z.n_dist;
     }
     return z;
 }
@@ -845,7 +951,7 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
 extern "C" int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table) {
     if (check_desc(d, "rgbd_attention_bwd_workspace")) return -1;
     const BwdSizes z = bwd_sizes(d, want_table && d->table);
-    return z.delta + z.part + z.by_dist + 4;
+    return z.delta + z.part + z.sums + 4;
 }
 
 extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream) {
@@ -878,29 +984,35 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
     a.delta = workspace;
     a.part = workspace + z.delta;
     a.span = z.span;
-    float* by_dist = a.part + z.part;
+    float* sums = a.part + z.part;
     const bool cap = d->cap > 0.f;
 
     if (d->Lq > 0) {
         const int bias = bias_mode(d, 0);
-        size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4 + (dt ? KT * BLK * 4 : 0);
+        size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4 + DT_LDS[z.mode];
         a.seg_tiles = 1;
         if (bias && d->Lk > 0) {
-            a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols);
+            // with the table's gradient a workgroup keeps to half of the compute unit's LDS where the head size lets it
+            a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols, z.mode ? 2304 : WIN_FLOATS);
             RGBD_REQUIRE(a.seg_tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
             lds += window_bytes(d->Lq, d->Lk, a.rows, a.cols, a.seg_tiles);
         }
         const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
-        const int rc = d->D == 32 ? launch_dq<32>(a, bias, cap, dt, grid, lds, s) : d->D == 64 ? launch_dq<64>(a, bias, cap, dt, grid, lds, s)
-                                                                                               : launch_dq<128>(a, bias, cap, dt, grid, lds, s);
+        const int rc = d->D == 32 ? launch_dq<32>(a, bias, cap, z.mode, grid, lds, s) : d->D == 64 ? launch_dq<64>(a, bias, cap, z.mode, grid, lds, s)
+                                                                                               : launch_dq<128>(a, bias, cap, z.mode, grid, lds, s);
         if (rc) return rc;
         RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dq)");
     }
-    if (dt && !empty) {
-        hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 256), 2 * a.H), dim3(256), 0, s, a, by_dist, z.n_dist, z.d0);
-        hipLaunchKernelGGL(attn_bucket_kernel, dim3(a.n_buckets, a.H), dim3(64), 0, s, a, by_dist, g->order, g->start, z.n_dist, z.d0);
-        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
+    if (z.mode == DT_BLOCKS) {
+        const int classes = (z.q_rows + z.k_rows - 1) * (z.gq + z.gk - 1);
+        hipLaunchKernelGGL(attn_block_sums_kernel, dim3(classes, a.H), dim3(1024), 0, s, a, sums, z.q_row0, z.q_rows, z.k_rows, z.gq, z.gk);
+        hipLaunchKernelGGL(attn_block_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.q_row0, z.k_rows,
+                           z.q_rows, z.gq, z.gk);
+    } else if (z.mode == DT_DIAGONALS) {
+        hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 64), 2 * a.H), dim3(1024), 0, s, a, sums, z.n_dist, z.d0);
+        hipLaunchKernelGGL(attn_dist_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.n_dist, z.d0);
     }
+    if (z.mode) RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
     if (d->Lk > 0) {
         const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
         size_t lds = 4 * KT * 2 * d->D + 6 * KT * 4;
