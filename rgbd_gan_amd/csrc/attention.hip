@@ -14,15 +14,20 @@
 // product as they stand (its K order follows the accumulator's: 4 keys of one half, 4 of the other), while the A operand comes
 // out of LDS through the transposing read.  Probabilities and score gradients are rounded to bf16 only as operands of these
 // products; maxima, sums, statistics and the table's gradient stay in fp32.
+#include <type_traits>
+
 #include "common.h"
 
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int KT = 64;                    // rows of a streamed tile (keys forward and in dq, queries in dk / dv)
+// rows of a streamed tile (keys forward and in dq, queries in dk / dv): two buffers of two operands are 32 KB of LDS either way
+constexpr int kt_of(int D) { return D == 128 ? 32 : 64; }
 constexpr int BLK = 128;                  // rows a workgroup owns: 4 waves x 32
-constexpr int WIN_FLOATS = 8192;          // LDS floats for a window of the bias (32 KB): it spans as many tiles as fit
 constexpr int WIN_PAD = 4;
+// LDS bytes for the window: next to the tiles of two workgroups of head size 64 (32 KB each, 69 KB with ds blocks) in 160 KB
+constexpr int WIN_FWD = 20480, WIN_DQ = 11264;
+constexpr float NO_ROW = 0x1p100f;          // log2-sum-exp of a row that is not there: p = exp2(x - 2^100) = 0 for every finite x
 constexpr float NEG_INF = -__builtin_inff();
 
 struct AttnArgs {
@@ -33,14 +38,16 @@ struct AttnArgs {
     int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
     int64_t dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
     int B, H, Hkv, rep, Lq, Lk;
-    int rows, cols, q_start, n_buckets;
-    int n_qb, n_kb, n_kt, seg_tiles;
+    int rows, cols, pos_cols, q_start, n_buckets;
+    int kt, n_qb, n_kb, n_kt, seg_tiles, win_bytes;
     int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
     float scale, cap;
 };
 
-// ---- positions
+// ---- positions.  `cols` here is pos_cols: the grid's columns, or a number no token reaches where the grid is a single row.
 __device__ __forceinline__ int pos_of(int t, int cols) { return t + (cols - 1) * (t / cols); }
+
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
 // ---- LDS tiles: `rows` x D bf16, 16-byte chunks permuted so that both ways of reading a tile spread over the 64 banks: the
 //      row-major 16-byte reads of 32 consecutive rows and the transposing 8-byte reads of 4 consecutive rows x 64 bytes.
@@ -77,27 +84,46 @@ template <int D> struct Frags {
     }
 };
 
-// One tile of KT rows x D from global memory into LDS through registers; rows at or beyond `valid` become zeros (whatever the
-// memory holds there, a NaN included).
-template <int D> struct Stage {
-    static constexpr int CH = D / 8, NP = KT * CH / 256;
-    u32x4 r[NP];
-    __device__ __forceinline__ void load(const unsigned short* base, int64_t sl, int row0, int valid) {
+// One tile of KT rows x D from global memory straight into LDS (global_load_lds: no registers, 16 bytes a lane, a wave's 1 KB in a
+// row; the permutation of the chunks is in the source addresses).  Rows at or beyond `valid` repeat the last valid one: whatever
+// memory holds there, a NaN included, is never read.  M0 carries the LDS address; nothing the compiler emits for gfx950 reads it.
+// The caller waits with dma_wait() before the barrier that publishes the tile.
+template <int D> struct Dma {
+    static constexpr int KT = kt_of(D), CH = D / 8, NP = KT * CH / 256;
+    unsigned off[NP];                     // bytes from the tile's first row
+    int64_t step;                         // bytes of KT rows
+    const char* base;
+    int valid;                            // rows from the next tile's first on
+    unsigned lds;
+    __device__ __forceinline__ void offsets(int64_t sl, int rows) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
-            const int pc = threadIdx.x + 256 * i, row = row0 + pc / CH, ch = pc % CH;
-            if (row < valid) r[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)row * sl + ch * 8);
-            else r[i] = u32x4{0, 0, 0, 0};
+            const int pc = threadIdx.x + 256 * i, row = pc / CH, ch = (pc % CH) ^ swz<D>(row);
+            off[i] = (unsigned)min(row, rows - 1) * (unsigned)(2 * sl) + 16 * ch;
         }
     }
-    __device__ __forceinline__ void store(char* tile) const {
+    __device__ __forceinline__ void init(const unsigned short* p, int64_t sl, int rows, const char* tile) {
+        base = reinterpret_cast<const char*>(p);
+        step = 2 * KT * sl;
+        valid = rows;
+        lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)tile + 1024 * wave_id();
+        offsets(sl, rows);
+    }
+    // the next tile, `buf_bytes` behind the first buffer
+    __device__ __forceinline__ void next(int64_t sl, int buf_bytes) {
+        if (valid < KT) offsets(sl, valid);
+        const uint64_t b = (uint64_t)(uintptr_t)base;                 // (uniform by construction; said so where the compiler lost it)
+        const uint64_t from = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((int)(b >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((int)b);
+        const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)lds) + buf_bytes;
 #pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            const int pc = threadIdx.x + 256 * i, row = pc / CH, ch = pc % CH;
-            *reinterpret_cast<u32x4*>(tile + row * (2 * D) + ((ch ^ swz<D>(row)) << 4)) = r[i];
-        }
+        for (int i = 0; i < NP; ++i)
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                         :: "s"(to + 4096 * i), "v"(off[i]), "s"(from) : "memory", "m0");
+        base += step;
+        valid -= KT;
     }
 };
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ f32x16 mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -111,11 +137,21 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& v, int i0) {
 __device__ __forceinline__ float other_half_max(float x) { return fmaxf(x, __shfl_xor(x, 32, 64)); }
 __device__ __forceinline__ float other_half_sum(float x) { return x + __shfl_xor(x, 32, 64); }
 
-__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 // LDS operations of one wave complete in order; this keeps the compiler to that order where lanes read what others wrote
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
+}
+
+// The loads of `f` are waited for here: left to the first use, inside the loop, that wait would also wait for the loop's own loads
+// of the next tile (one counter, in order) -- which doubled the time of a tile.
+template <int N> __device__ __forceinline__ void arrived(bf16x8 (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        u32x4 v = __builtin_bit_cast(u32x4, f[i]);
+        asm volatile("" : "+v"(v));
+        f[i] = __builtin_bit_cast(bf16x8, v);
+    }
 }
 
 // tanh of 16 values.  Below 0.5 an odd polynomial (least squares on Chebyshev nodes, relative error 1.1e-7: there the quotient
@@ -152,59 +188,125 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
     return x * q + min(x, r) + (id >> 3);
 }
 
-// ---- the bias of a run of tiles, in LDS.  `own` = the workgroup's rows (first P, last P), `other` = the streamed rows.  Entry j is
-//      the offset whose place grows with the streamed row, so a lane reads upwards; SIGN: +1 streamed rows are queries.
-//      Values are kept times log2(e): the softmax runs on exp2.
+// ---- the bias of a run of tiles (a segment), in LDS.  The workgroup's own rows are tokens at places own_first .. own_last, the
+//      streamed ones begin at other_first and span `span` places.  Entry j is the offset whose place grows with the streamed row, so a
+//      lane reads upwards; SIGN +1: the streamed rows are queries.  Values are kept times log2(e): the softmax runs on exp2.
 template <int SIGN>
-__device__ __forceinline__ void stage_window(float* win, const AttnArgs& a, int h, int own_first, int own_last, int other_first,
-                                             int other_last) {
-    const int n = (own_last - own_first) + (other_last - other_first) + 1;
-    const int c0 = (2 * a.cols - 1) * (a.rows - 1) + a.cols - 1;
+__device__ __forceinline__ void stage_window(float* win, const AttnArgs& a, int h, int own_first, int own_last, int other_first, int span) {
+    const int n = (own_last - own_first) + span + 1 + WIN_PAD;
+    const int c0 = (2 * a.cols - 1) * (a.rows - 1) + a.cols - 1, size = (2 * a.cols - 1) * (2 * a.rows - 1);
     const float* row = a.table + (int64_t)h * a.n_buckets;
     const int base = SIGN > 0 ? other_first - own_last + c0 : own_last - other_first + c0;
     for (int j = threadIdx.x; j < n; j += 256) {
-        int u = a.map[base + SIGN * j];
-        u = min(max(u, 0), a.n_buckets - 1);
-        win[j] = row[u] * LOG2E;
+        const int e = base + SIGN * j;                                // beyond the map: a streamed row that is no token
+        const int u = min(max(a.map[min(max(e, 0), size - 1)], 0), a.n_buckets - 1);
+        win[j] = e >= 0 && e < size ? row[u] * LOG2E : 0.f;
     }
-    if (threadIdx.x < WIN_PAD) win[n + threadIdx.x] = 0.f;            // a group of four at the end of the tokens reads past them
 }
 
-// 16 biases of a lane: rows 32 s + 8 (i / 4) + 4 half + i % 4 of the streamed tile; `at` = 64 window places (bytes) of the tile.
-// BIAS 2: four aligned rows of the tile are neighbours in the window (one row of the grid), BIAS 1: any.
-template <int BIAS>
-__device__ __forceinline__ void read_bias(f32x16& o, const char* win, const int* at, int s, int half, int lane_off) {
+// Where in the window the streamed rows of a block of 32 lie, in bytes, from the segment's first on.
+// BIAS 2 (regular grids): a block's four groups of 8 rows lie at distances that are the same for every block, the rows of a half of
+// a group are neighbours, and from block to block the place grows by a fixed step (rows of the grid divide 32) or by 32 and, at the
+// end of a row of the grid, by columns - 1 more: a handful of scalars.  BIAS 1 (any grid): a table of the segment's rows.
+template <int BIAS> struct Places {
+    int blk, x, step, wrap, cols, g[4];
+    __device__ __forceinline__ void init(const AttnArgs& a, int first) {
+        if (BIAS != 2) return;
+        const bool narrow = a.rows > 1 && a.cols < 32;
+        blk = 0;
+        cols = a.pos_cols;
+        x = narrow ? 0 : first % cols;
+        step = 4 * (narrow ? 32 + 32 / a.cols * (a.cols - 1) : 32);
+        wrap = narrow ? 0 : 4 * (cols - 1);
+        if (narrow) cols = 1 << 30;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int* p = at + 32 * s + 8 * g + 4 * half;
-        if (BIAS == 2) {
-            const float* w = reinterpret_cast<const float*>(win + p[0] + lane_off);
+        for (int i = 0; i < 4; ++i) g[i] = 4 * (8 * i + (narrow ? (a.cols - 1) * (8 * i / a.cols) : 0));
+    }
+    // bytes from a lane's own place: rows 4 half .. 4 half + 3 of a group
+    static __device__ __forceinline__ int half_off(const AttnArgs& a, int half) {
+        return BIAS == 2 ? 4 * (4 * half + (a.rows > 1 && a.cols == 4 ? 3 * half : 0)) : 0;
+    }
+    __device__ __forceinline__ void next() {
+        if (BIAS != 2) return;
+        blk += step;
+        x += 32;
+        if (x >= cols) { x -= cols; blk += wrap; }
+    }
+    // the table of BIAS 1: places of the segment's rows (tokens first .. first + n - 1, repeated from the last that exists on)
+    static __device__ __forceinline__ void table(int* at, const AttnArgs& a, int first, int n, int last) {
+        if (BIAS != 1) return;
+        const int p0 = pos_of(first, a.pos_cols);
+        for (int i = threadIdx.x; i < n; i += 256) at[i] = 4 * (pos_of(min(first + i, last), a.pos_cols) - p0);
+    }
+};
+
+// 16 biases of a lane: rows 8 (i / 4) + 4 half + i % 4 of a block of 32; `at`: the block's rows in the table of BIAS 1.
+template <int BIAS>
+__device__ __forceinline__ f32x16 read_bias(const char* win, const Places<BIAS>& pl, const int* at, int half, int lane_off) {
+    f32x16 o;
+    if (BIAS == 0) return o;
+    if (BIAS == 2) {
+        const char* w0 = win + (lane_off + pl.blk);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const float* w = reinterpret_cast<const float*>(w0 + pl.g[g]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[4 * g + i] = w[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[4 * g + i] = *reinterpret_cast<const float*>(win + p[i] + lane_off);
         }
+    } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[4 * g + i] = *reinterpret_cast<const float*>(win + at[8 * g + 4 * half + i] + lane_off);
     }
+    return o;
 }
 
-// Scores of 16 (lane, streamed row) pairs in units of log2: raw products in, tanh part kept in `th` where asked.
+// Scores of 16 (lane, streamed row) pairs in units of log2, from raw products (which may carry a constant in units of 1 / f).
+// With a cap the tanh stays in `th`.
 template <int BIAS, bool CAP>
-__device__ __forceinline__ void to_logits(f32x16& x, f32x16& th, const AttnArgs& a, const char* win, const int* at, int s, int half,
-                                          int lane_off) {
-    f32x16 bias;
-    if (BIAS) read_bias<BIAS>(bias, win, at, s, half, lane_off);
+__device__ __forceinline__ void to_logits(f32x16& x, f32x16& th, const AttnArgs& a, const f32x16& bias) {
     if (CAP) {
         th = x;
         tanh16(th, a.scale / a.cap);
-        const float f = a.cap * LOG2E;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = BIAS ? th[i] * f + bias[i] : th[i] * f;
-    } else {
-        const float f = a.scale * LOG2E;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = BIAS ? x[i] * f + bias[i] : x[i] * f;
     }
+    const float f = CAP ? a.cap * LOG2E : a.scale * LOG2E;
+    const f32x16& r = CAP ? th : x;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = BIAS ? r[i] * f + bias[i] : r[i] * f;
+}
+
+// Operands of a block of 32 streamed rows, read as a group ahead of their use: the compiler, left alone, reads each next to its
+// matrix instruction and waits out the LDS latency every time.
+template <int D> struct RowOps {
+    bf16x8 f[D / 16];
+    __device__ __forceinline__ void load(const Frags<D>& fr, const char* tile, int row0) {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) f[ks] = fr.row(tile, row0, ks);
+    }
+    // products with the workgroup's own 32 rows (a lane each), from c on
+    __device__ __forceinline__ f32x16 times(const bf16x8* own, f32x16 c) const {
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ++ks) c = mfma(f[ks], own[ks], c);
+        return c;
+    }
+};
+template <int D> struct ColOps {
+    bf16x8 f[2][D / 32];
+    __device__ __forceinline__ void load(const Frags<D>& fr, const char* tile, int row0) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d) f[g][d] = fr.col(tile, row0 + 16 * g, d);
+    }
+};
+#define PHASE() __builtin_amdgcn_sched_barrier(0)
+
+__device__ __forceinline__ f32x16 splat(float v) {
+    f32x16 r;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) r[i] = v;
+    return r;
 }
 
 __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
@@ -212,17 +314,15 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 }
 
 // ======================================================================================================= forward
-// LDS: K[2] V[2] tiles | at[2][64] | window.
+// LDS: K[2] V[2] tiles | window | table of the segment's places (BIAS 1).
 // FINE: the probabilities go into the second product as two bf16 terms (16 bits): delta = do . o must be that exact where the
-// fp32 gradient of the table is wanted (with one term it is off by 5e-4, with two by 3e-6); V's fragments serve both.
+// fp32 gradient of the table is wanted (with one term it is off by 5e-4, with two by 3e-6); V's operands serve both.
 template <int D, int BIAS, bool CAP, bool FINE>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
-    char* kt = smem;
-    char* vt = smem + 2 * TB;
-    int* at = reinterpret_cast<int*>(smem + 4 * TB);
-    float* win = reinterpret_cast<float*>(smem + 4 * TB + 2 * KT * 4);
+    constexpr int KT = kt_of(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    char* win = smem + 4 * TB;
+    int* at = reinterpret_cast<int*>(win + a.win_bytes);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
     const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
@@ -242,103 +342,132 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
     const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
 
     const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
-    const int pq0 = BIAS ? pos_of(tq0, a.cols) : 0, pq1 = BIAS ? pos_of(tq1, a.cols) : 0;
-    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.cols)) : 0;
+    const int pq0 = BIAS ? pos_of(tq0, a.pos_cols) : 0, pq1 = BIAS ? pos_of(tq1, a.pos_cols) : 0;
+    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.pos_cols)) + Places<BIAS>::half_off(a, half) : 0;
 
     f32x16 o[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-    float m = NEG_INF, l = 0.f;
+    for (int d = 0; d < DB; ++d) o[d] = splat(0.f);
+    // The softmax's reference m: probabilities are exp2(x - m).  fp32 sums and bf16 operands keep their digits at any scale, so m stays
+    // 0 while the sums stay between 2^-80 and 2^60, and no maximum is looked for; a row that leaves this range takes its block's
+    // maximum as m (and scales what it has).
+    float m = 0.f, l = 0.f;
+    bool moved = false;                                              // (of the wave) some m is not 0
 
-    Stage<D> sk, sv;
-    auto places = [&](int t) {                                       // window places of tile t's keys, relative to its segment
-        if (BIAS && threadIdx.x < KT) {
-            const int seg0 = pos_of(t / a.seg_tiles * a.seg_tiles * KT, a.cols);
-            at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(min(t * KT + (int)threadIdx.x, a.Lk - 1), a.cols) - seg0);
-        }
-    };
+    Dma<D> sk, sv;
+    Places<BIAS> pl;
+    int seg_t = 0;                                                   // the first tile of the segment in the window
+    if (BIAS) pl.init(a, 0);
     if (nt > 0) {
-        sk.load(kp, a.k_sl, 0, len);
-        sv.load(vp, a.v_sl, 0, len);
-        sk.store(kt);
-        sv.store(vt);
-        places(0);
+        sk.init(kp, a.k_sl, len, smem);
+        sv.init(vp, a.v_sl, len, smem + 2 * TB);
+        sk.next(a.k_sl, 0);
+        sv.next(a.v_sl, 0);
+        dma_wait();
     }
-    for (int t = 0; t < nt; ++t) {
-        if (BIAS && t % a.seg_tiles == 0) {
+    arrived(qf);
+    auto tile = [&](int t, auto parity) {
+        constexpr int P = decltype(parity)::value;
+        const char* kc = smem + P * TB;
+        const char* vc = smem + (2 + P) * TB;
+        if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
             __syncthreads();                                         // every wave is done with the last window
-            const int last = min((t + a.seg_tiles) * KT, a.Lk) - 1;
-            stage_window<-1>(win, a, h, pq0, pq1, pos_of(t * KT, a.cols), pos_of(last, a.cols));
+            seg_t = t;
+            pl.blk = 0;
+            const int n = a.seg_tiles * KT, p0 = pos_of(t * KT, a.pos_cols);
+            stage_window<-1>(reinterpret_cast<float*>(win), a, h, pq0, pq1, p0, pos_of(t * KT + n - 1, a.pos_cols) - p0);
+            Places<BIAS>::table(at, a, t * KT, n, a.Lk - 1);
         }
         __syncthreads();
-        const char* kc = kt + (t & 1) * TB;
-        const char* vc = vt + (t & 1) * TB;
         if (t + 1 < nt) {
-            sk.load(kp, a.k_sl, (t + 1) * KT, len);
-            sv.load(vp, a.v_sl, (t + 1) * KT, len);
+            sk.next(a.k_sl, (P ^ 1) * TB);
+            sv.next(a.v_sl, (P ^ 1) * TB);
         }
-        f32x16 s[2], th;
+        PHASE();
+        f32x16 x, th;
+        const int* at_t = at + (t - seg_t) * KT;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < KT / 32; ++u) {
+            RowOps<D> kf;
+            kf.load(fr, kc, 32 * u);
+            const f32x16 bias = read_bias<BIAS>(win, pl, at_t + 32 * u, half, lane_off);
+            if (BIAS) pl.next();
+            PHASE();
+            x = kf.times(qf, splat(0.f));
+            ColOps<D> vf;
+            vf.load(fr, vc, 32 * u);
+            PHASE();
+            auto logits = [&] {
+                to_logits<BIAS, CAP>(x, th, a, bias);
+                if (t * KT + KT > len) {
+                    int k0 = t * KT + 32 * u + 4 * half;
+                    asm volatile("" : "+v"(k0));                     // (else the comparisons' operands are computed for every tile)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+                    for (int i = 0; i < 16; ++i)
+                        if (k0 + 8 * (i >> 2) + (i & 3) >= len) x[i] = NEG_INF;
+                }
+            };
+            logits();
+            if (moved)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s[u] = mfma(fr.row(kc, 32 * u, ks), qf[ks], s[u]);
-        }
-        float mx = NEG_INF;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            to_logits<BIAS, CAP>(s[u], th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
-            if (t * KT + KT > len) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (t * KT + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3) >= len) s[u][i] = NEG_INF;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-        }
-        mx = other_half_max(mx);
-        // the reference value follows the maximum only when it falls 2^8 behind: probabilities up to 2^8 lose nothing in bf16 or
-        // in the fp32 sums, and most tiles then skip the rescaling
-        if (__any(mx > m + 8.f)) {
-            const float mn = fmaxf(m, mx);
-            const float al = __builtin_amdgcn_exp2f(m - (mn == NEG_INF ? 0.f : mn));
-            m = mn;
-            l *= al;
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[d][i] *= al;
-        }
-        const float ms = m == NEG_INF ? 0.f : m;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
+                for (int i = 0; i < 16; ++i) x[i] -= m;
+            float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - ms);
-                l += s[u][i];
+                x[i] = __builtin_amdgcn_exp2f(x[i]);
+                sum += x[i];
             }
+            float ln = l + sum;
+            if (__any(!(ln > 0x1p-80f && ln < 0x1p60f))) {           // (a NaN comes here too, and stays one)
+                const float both = other_half_sum(ln);
+                const bool bad = !(both > 0x1p-80f && both < 0x1p60f);
+                if (__any(bad)) {
+                    kf.load(fr, kc, 32 * u);
+                    x = kf.times(qf, splat(0.f));
+                    logits();
+                    float top = NEG_INF;
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const bf16x8 pf = pack8(s[g >> 1], 8 * (g & 1));
+                    for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
+                    top = other_half_max(top);
+                    const float have = other_half_sum(l);
+                    float mn = have > 0.f ? fmaxf(m, top) : top;
+                    if (!bad || mn == NEG_INF) mn = m;
+                    const float al = have > 0.f ? __builtin_amdgcn_exp2f(m - mn) : (have == 0.f ? 0.f : have);
+                    m = mn;
+                    moved = true;
+                    sum = 0.f;
 #pragma unroll
-            for (int d = 0; d < DB; ++d) o[d] = mfma(fr.col(vc, 16 * g, d), pf, o[d]);
-            if (FINE) {
-                f32x16& p = s[g >> 1];
+                    for (int i = 0; i < 16; ++i) {
+                        x[i] = __builtin_amdgcn_exp2f(x[i] - m);
+                        sum += x[i];
+                    }
+                    ln = l * al + sum;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) p[8 * (g & 1) + i] -= (float)pf[i];
-                const bf16x8 pl = pack8(p, 8 * (g & 1));
+                    for (int d = 0; d < DB; ++d)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mfma(fr.col(vc, 16 * g, d), pl, o[d]);
+                        for (int i = 0; i < 16; ++i) o[d][i] *= al;
+                }
+            }
+            l = ln;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bf16x8 pf = pack8(x, 8 * g);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = mfma(vf.f[g][d], pf, o[d]);
+                if (FINE) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[8 * g + i] -= (float)pf[i];
+                    const bf16x8 pl2 = pack8(x, 8 * g);
+#pragma unroll
+                    for (int d = 0; d < DB; ++d) o[d] = mfma(vf.f[g][d], pl2, o[d]);
+                }
             }
         }
-        if (t + 1 < nt) {
-            sk.store(kt + ((t + 1) & 1) * TB);
-            sv.store(vt + ((t + 1) & 1) * TB);
-            places(t + 1);
-        }
+        dma_wait();
+    };
+    for (int t = 0; t < nt; t += 2) {
+        tile(t, std::integral_constant<int, 0>{});
+        if (t + 1 < nt) tile(t + 1, std::integral_constant<int, 1>{});
     }
     l = other_half_sum(l);
     if (row >= a.Lq) return;
@@ -372,23 +501,21 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(AttnArgs a) {
 //             whole kernel's time: 728 us against 264 with diagonals at 32 samples x 4 heads x 1024 tokens.)
 //   DIAGONALS any other grid: a pair is known by its distance i - j and by whether the column of i wraps (class 0: dx >= 0, class 1:
 //             dx < 0).  ds goes through LDS and a thread adds up one diagonal of the tile; a diagonal stays with its thread (distance
-//             mod 256) over the three tiles it crosses and is stored once: part (b, h, query block, class, distance).
-// LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (64 x 128 floats) | window.
+//             mod 256) over the tiles it crosses and is stored once: part (b, h, query block, class, distance).
+// LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
 enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
 constexpr int BS = 72;                    // floats from row to row of a block: rows 4 apart (a wave's halves) are 32 banks apart
 constexpr int BLOCK_FLOATS = 32 + 32 * BS;
-constexpr int DT_LDS[3] = {0, 4 * BLOCK_FLOATS * 4, KT * BLK * 4};
+constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * BLOCK_FLOATS * 4 : dt == DT_DIAGONALS ? kt_of(D) * BLK * 4 : 0; }
 
 template <int D, int BIAS, bool CAP, int DT>
-__global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
-    char* kt = smem;
-    char* vt = smem + 2 * TB;
-    int* at = reinterpret_cast<int*>(smem + 4 * TB);
-    float* dsl = reinterpret_cast<float*>(smem + 4 * TB + 2 * KT * 4);
-    float* win = dsl + DT_LDS[DT] / 4;
-    const int n_kg = a.n_kt * 2;
+    constexpr int KT = kt_of(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    float* dsl = reinterpret_cast<float*>(smem + 4 * TB);
+    char* win = smem + 4 * TB + dt_lds(DT, D);
+    int* at = reinterpret_cast<int*>(win + a.win_bytes);
+    const int n_kg = a.n_kt * (KT / 32);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
     const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
@@ -421,69 +548,77 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
     delta = other_half_sum(delta);
     if (live && half == 0) a.delta[(int64_t)bh * a.Lq + row] = delta;
     if (!live) delta = 0.f;
-    const float lse = live ? a.lse[(int64_t)bh * a.Lq + row] : __builtin_inff();      // a row that is not there has p = 0
+    const float lse = live ? a.lse[(int64_t)bh * a.Lq + row] : NO_ROW;
 
     const int len = keys_of(a, b);
     const int nt = (len + KT - 1) / KT;
     const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
     const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
     const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
-    const int pq0 = BIAS ? pos_of(tq0, a.cols) : 0, pq1 = BIAS ? pos_of(tq1, a.cols) : 0;
-    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.cols)) : 0;
+    const int pq0 = BIAS ? pos_of(tq0, a.pos_cols) : 0, pq1 = BIAS ? pos_of(tq1, a.pos_cols) : 0;
+    const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.pos_cols)) + Places<BIAS>::half_off(a, half) : 0;
 
     f32x16 acc[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+    for (int d = 0; d < DB; ++d) acc[d] = splat(0.f);
     float sum0 = 0.f, sum1 = 0.f;                                    // the thread's diagonal, by class
     // DIAGONALS: partials of this workgroup, place 0 = the smallest distance it meets
     float* part = DT == DT_DIAGONALS ? a.part + (int64_t)id * 2 * a.span
                                      : DT == DT_BLOCKS ? a.part + ((int64_t)id * 4 + wave) * n_kg * 64 : nullptr;
     const int d_min = tq0 - (nt * KT - 1);
 
-    Stage<D> sk, sv;
-    auto places = [&](int t) {
-        if (BIAS && threadIdx.x < KT) {
-            const int seg0 = pos_of(t / a.seg_tiles * a.seg_tiles * KT, a.cols);
-            at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(min(t * KT + (int)threadIdx.x, a.Lk - 1), a.cols) - seg0);
-        }
-    };
+    Dma<D> sk, sv;
+    Places<BIAS> pl;
+    int seg_t = 0;
+    if (BIAS) pl.init(a, 0);
     if (nt > 0) {
-        sk.load(kp, a.k_sl, 0, len);
-        sv.load(vp, a.v_sl, 0, len);
-        sk.store(kt);
-        sv.store(vt);
-        places(0);
+        sk.init(kp, a.k_sl, len, smem);
+        sv.init(vp, a.v_sl, len, smem + 2 * TB);
+        sk.next(a.k_sl, 0);
+        sv.next(a.v_sl, 0);
+        dma_wait();
     }
-    for (int t = 0; t < nt; ++t) {
-        if (BIAS && t % a.seg_tiles == 0) {
+    arrived(qf);
+    arrived(gf);
+    auto tile = [&](int t, auto parity) {
+        constexpr int P = decltype(parity)::value;
+        const char* kc = smem + P * TB;
+        const char* vc = smem + (2 + P) * TB;
+        if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
             __syncthreads();
-            const int last = min((t + a.seg_tiles) * KT, a.Lk) - 1;
-            stage_window<-1>(win, a, h, pq0, pq1, pos_of(t * KT, a.cols), pos_of(last, a.cols));
+            seg_t = t;
+            pl.blk = 0;
+            const int n = a.seg_tiles * KT, p0 = pos_of(t * KT, a.pos_cols);
+            stage_window<-1>(reinterpret_cast<float*>(win), a, h, pq0, pq1, p0, pos_of(t * KT + n - 1, a.pos_cols) - p0);
+            Places<BIAS>::table(at, a, t * KT, n, a.Lk - 1);
         }
         __syncthreads();
-        const char* kc = kt + (t & 1) * TB;
-        const char* vc = vt + (t & 1) * TB;
         if (t + 1 < nt) {
-            sk.load(kp, a.k_sl, (t + 1) * KT, len);
-            sv.load(vp, a.v_sl, (t + 1) * KT, len);
+            sk.next(a.k_sl, (P ^ 1) * TB);
+            sv.next(a.v_sl, (P ^ 1) * TB);
         }
+        PHASE();
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f32x16 s, dp, th;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                s = mfma(fr.row(kc, 32 * u, ks), qf[ks], s);
-                dp = mfma(fr.row(vc, 32 * u, ks), gf[ks], dp);
-            }
-            to_logits<BIAS, CAP>(s, th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
+        for (int u = 0; u < KT / 32; ++u) {
+            RowOps<D> f;
+            f.load(fr, kc, 32 * u);
+            PHASE();
+            f32x16 s = f.times(qf, splat(0.f)), th;
+            f.load(fr, vc, 32 * u);
+            const f32x16 bias = read_bias<BIAS>(win, pl, at + (t - seg_t) * KT + 32 * u, half, lane_off);
+            if (BIAS) pl.next();
+            PHASE();
+            f32x16 dp = f.times(gf, splat(0.f));
+            ColOps<D> kt;
+            kt.load(fr, kc, 32 * u);
+            PHASE();
+            to_logits<BIAS, CAP>(s, th, a, bias);
             if (t * KT + KT > len) {
+                int k0 = t * KT + 32 * u + 4 * half;
+                asm volatile("" : "+v"(k0));
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (t * KT + 32 * u + 8 * (i >> 2) + 4 * half + (i & 3) >= len) s[i] = NEG_INF;
+                    if (k0 + 8 * (i >> 2) + (i & 3) >= len) s[i] = NEG_INF;
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -492,26 +627,22 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                 if (DT == DT_BLOCKS) blk[(8 * (i >> 2) + 4 * half + (i & 3)) * BS + (lane & 31)] = ds;
                 s[i] = CAP ? ds * (1.f - th[i] * th[i]) : ds;
             }
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                const bf16x8 pf = pack8(s, 8 * g);
+#pragma unroll
+                for (int d = 0; d < DB; ++d) acc[d] = mfma(kt.f[g][d], pf, acc[d]);
+            }
             if (DT == DT_BLOCKS) {                                   // lane: query - key = lane - 32
                 wave_fence();
                 float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) sum += blk[i * (BS + 1) + lane - 32];
-                part[(2 * t + u) * 64 + lane] = sum;
+                part[(KT / 32 * t + u) * 64 + lane] = sum;
                 wave_fence();
             }
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                const bf16x8 pf = pack8(s, 8 * g);
-#pragma unroll
-                for (int d = 0; d < DB; ++d) acc[d] = mfma(fr.col(kc, 32 * u + 16 * g, d), pf, acc[d]);
-            }
         }
-        if (t + 1 < nt) {
-            sk.store(kt + ((t + 1) & 1) * TB);
-            sv.store(vt + ((t + 1) & 1) * TB);
-            places(t + 1);
-        }
+        dma_wait();
         if (DT == DT_DIAGONALS) {
             __syncthreads();
             const int k0 = t * KT, lo = tq0 - k0 - (KT - 1);         // smallest distance of this tile
@@ -536,13 +667,17 @@ __global__ __launch_bounds__(256, 2) void attn_dq_kernel(AttnArgs a) {
                         x -= x == r ? a.cols : 0;                    // the key's own row ends
                     }
                 }
-                if (c >= KT || t + 1 == nt) {                        // the diagonal leaves the workgroup's rows
+                if (c + KT >= BLK || t + 1 == nt) {                        // the diagonal leaves the workgroup's rows
                     part[dist - d_min] = sum0;
                     part[a.span + dist - d_min] = sum1;
                     sum0 = sum1 = 0.f;
                 }
             }
         }
+    };
+    for (int t = 0; t < nt; t += 2) {
+        tile(t, std::integral_constant<int, 0>{});
+        if (t + 1 < nt) tile(t + 1, std::integral_constant<int, 1>{});
     }
     if (!live) return;
     unsigned short* qo = a.dq + b * a.dq_sb + (int64_t)row * a.dq_sl + h * a.dq_sh + 4 * half;
@@ -566,12 +701,12 @@ __global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float
     const int dy = cls / dgs - (k_rows - 1), dg = cls % dgs - (gk - 1);       // query group row (from q_row0) - key row, group - group
     const int y0 = max(0, dy), y1 = min(q_rows, k_rows + dy), g0 = max(0, dg), g1 = min(gq, gk + dg);
     const int ny = max(0, y1 - y0), ng = max(0, g1 - g0), n = a.B * ny * ng;
-    const int n_qg = a.n_qb * 4, n_kg = a.n_kt * 2;
+    const int n_qg = a.n_qb * 4, n_kg = a.n_kt * (a.kt / 32);
     float s = 0.f;
     for (int e = r; e < n; e += 16) {
         const int g = g0 + e % ng, y = y0 + e / ng % ny, b = e / (ng * ny);
         const int qg = y * gq + g, kg = (y - dy) * gk + g - dg;
-        if (qg >= n_qg || kg >= 2 * ((keys_of(a, b) + KT - 1) / KT)) continue;
+        if (qg >= n_qg || kg >= a.kt / 32 * ((keys_of(a, b) + a.kt - 1) / a.kt)) continue;
         s += a.part[((int64_t)((b * a.H + h) * n_qg + qg) * n_kg + kg) * 64 + lane];
     }
     red[threadIdx.x] = s;
@@ -616,8 +751,8 @@ __global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_d
     float s = 0.f;
     for (int e = r; e < a.B * a.n_qb; e += 16) {
         const int qb = e % a.n_qb, b = e / a.n_qb;
-        const int nt = (keys_of(a, b) + KT - 1) / KT;
-        const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * KT - 1));
+        const int nt = (keys_of(a, b) + a.kt - 1) / a.kt;
+        const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * a.kt - 1));
         if (nt == 0 || place < 0 || dist > tq0 + BLK - 1) continue;
         s += a.part[((int64_t)((b * a.H + h) * a.n_qb + qb) * 2 + cls) * a.span + place];
     }
@@ -649,17 +784,15 @@ __global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const
 // ======================================================================================================= dk, dv
 // A workgroup owns 128 keys of one key / value head and streams the queries of every head that shares it: scores here are
 // queries x keys, a lane holds one key.  No sum leaves the workgroup.
-// LDS: Q[2] dO[2] | at[2][64] | lse[2][64] | delta[2][64] | window.
+// LDS: Q[2] dO[2] | lse[2][64] | delta[2][64] | window | table of the segment's places (BIAS 1).
 template <int D, int BIAS, bool CAP>
-__global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int TB = KT * 2 * D, KS = D / 16, DB = D / 32;
-    char* qt = smem;
-    char* gt = smem + 2 * TB;
-    int* at = reinterpret_cast<int*>(smem + 4 * TB);
-    float* ls = reinterpret_cast<float*>(at + 2 * KT);
+    constexpr int KT = kt_of(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    float* ls = reinterpret_cast<float*>(smem + 4 * TB);
     float* dl = ls + 2 * KT;
-    float* win = dl + 2 * KT;
+    char* win = reinterpret_cast<char*>(dl + 2 * KT);
+    int* at = reinterpret_cast<int*>(win + a.win_bytes);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
     const int kb = id % a.n_kb, bk = id / a.n_kb, hk = bk % a.Hkv, b = bk / a.Hkv;
@@ -670,9 +803,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
 
     f32x16 dk[DB], dv[DB];
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) dk[d][i] = dv[d][i] = 0.f;
+    for (int d = 0; d < DB; ++d) dk[d] = dv[d] = splat(0.f);
 
     if (kb * BLK < len && a.Lq > 0) {
         bf16x8 kf[KS], vf[KS];
@@ -687,85 +818,112 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
             }
         }
         const int tk0 = kb * BLK, tk1 = min(kb * BLK + BLK, a.Lk) - 1;
-        const int pk0 = BIAS ? pos_of(tk0, a.cols) : 0, pk1 = BIAS ? pos_of(tk1, a.cols) : 0;
-        const int lane_off = BIAS ? 4 * (pk1 - pos_of(min(key, tk1), a.cols)) : 0;
-        const int nqt = (a.Lq + KT - 1) / KT, nt = nqt * a.rep;
+        const int pk0 = BIAS ? pos_of(tk0, a.pos_cols) : 0, pk1 = BIAS ? pos_of(tk1, a.pos_cols) : 0;
+        const int lane_off = BIAS ? 4 * (pk1 - pos_of(min(key, tk1), a.pos_cols)) + Places<BIAS>::half_off(a, half) : 0;
+        const int nqt = (a.Lq + KT - 1) / KT;
+        const float neg_inv_f = -1.f / (a.scale * LOG2E);
 
-        Stage<D> sq, sg;
+        Dma<D> sq, sg;
         float next_l = 0.f, next_d = 0.f;
-        auto load = [&](int t) {
-            const int h = hk * a.rep + t / nqt, r0 = t % nqt * KT;
-            sq.load(a.q + b * a.q_sb + h * a.q_sh, a.q_sl, r0, a.Lq);
-            sg.load(a.d_o + ((int64_t)b * a.Lq * a.H + h) * D, (int64_t)a.H * D, r0, a.Lq);
+        auto load = [&](int h, int t, int buf) {                      // tile t of head h into buffer buf
+            if (t == 0) {
+                sq.init(a.q + b * a.q_sb + h * a.q_sh, a.q_sl, a.Lq, smem);
+                sg.init(a.d_o + ((int64_t)b * a.Lq * a.H + h) * D, (int64_t)a.H * D, a.Lq, smem + 2 * TB);
+            }
+            sq.next(a.q_sl, buf * TB);
+            sg.next((int64_t)a.H * D, buf * TB);
             if (threadIdx.x < KT) {
-                const int r = r0 + threadIdx.x;
+                const int r = t * KT + threadIdx.x;
                 const int64_t at_row = (int64_t)(b * a.H + h) * a.Lq + r;
-                next_l = r < a.Lq ? a.lse[at_row] : __builtin_inff();
+                next_l = r < a.Lq ? a.lse[at_row] : NO_ROW;
                 next_d = r < a.Lq ? a.delta[at_row] : 0.f;
             }
         };
-        auto store = [&](int t) {
-            sq.store(qt + (t & 1) * TB);
-            sg.store(gt + (t & 1) * TB);
+        auto store = [&](int p) {
             if (threadIdx.x < KT) {
-                ls[(t & 1) * KT + threadIdx.x] = next_l;
-                dl[(t & 1) * KT + threadIdx.x] = next_d;
-                if (BIAS) {
-                    const int tt = t % nqt, seg0 = a.q_start + tt / a.seg_tiles * a.seg_tiles * KT;
-                    const int tok = a.q_start + min(tt * KT + (int)threadIdx.x, a.Lq - 1);
-                    at[(t & 1) * KT + threadIdx.x] = 4 * (pos_of(tok, a.cols) - pos_of(seg0, a.cols));
-                }
+                ls[p * KT + threadIdx.x] = CAP ? next_l : next_l * neg_inv_f;     // the scores' products start from -lse / f
+                dl[p * KT + threadIdx.x] = -next_d;                               // ... and dp's from -delta
             }
+            dma_wait();
         };
-        load(0);
+        Places<BIAS> pl;
+        int h = hk * a.rep, t = 0, seg_t = 0;                        // the tile at hand: head, tile of its queries
+        load(h, 0, 0);
         store(0);
-        for (int t = 0; t < nt; ++t) {
-            const int tt = t % nqt;
-            if (BIAS && tt % a.seg_tiles == 0) {
+        arrived(kf);
+        arrived(vf);
+        const int n_all = nqt * a.rep;
+        auto tile = [&](int n, auto parity) {
+            constexpr int P = decltype(parity)::value;
+            const char* qc = smem + P * TB;
+            const char* gc = smem + (2 + P) * TB;
+            const float* lc = ls + P * KT;
+            const float* dc = dl + P * KT;
+            if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
                 __syncthreads();
-                const int last = a.q_start + min((tt + a.seg_tiles) * KT, a.Lq) - 1;
-                stage_window<1>(win, a, hk * a.rep + t / nqt, pk0, pk1, pos_of(a.q_start + tt * KT, a.cols), pos_of(last, a.cols));
+                if (t == 0) pl.init(a, a.q_start);
+                seg_t = t;
+                pl.blk = 0;
+                const int rows = a.seg_tiles * KT, first = a.q_start + t * KT, p0 = pos_of(first, a.pos_cols);
+                stage_window<1>(reinterpret_cast<float*>(win), a, h, pk0, pk1, p0, pos_of(first + rows - 1, a.pos_cols) - p0);
+                Places<BIAS>::table(at, a, first, rows, a.q_start + a.Lq - 1);
             }
             __syncthreads();
-            const char* qc = qt + (t & 1) * TB;
-            const char* gc = gt + (t & 1) * TB;
-            const float* lc = ls + (t & 1) * KT;
-            const float* dc = dl + (t & 1) * KT;
-            if (t + 1 < nt) load(t + 1);
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                f32x16 s, dp, th;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s[i] = dp[i] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    s = mfma(fr.row(qc, 32 * u, ks), kf[ks], s);
-                    dp = mfma(fr.row(gc, 32 * u, ks), vf[ks], dp);
-                }
-                to_logits<BIAS, CAP>(s, th, a, reinterpret_cast<const char*>(win), at + (t & 1) * KT, u, half, lane_off);
+            const int* at_t = at + (t - seg_t) * KT;
+            if (++t == nqt) { t = 0; ++h; }
+            if (n + 1 < n_all) load(h, t, P ^ 1);
+            PHASE();
+            auto rows16 = [&](const float* v, int u) {                // a value per streamed row of the block, as the products lie
+                f32x16 r;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(lc + 32 * u + 8 * g + 4 * half);
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(dc + 32 * u + 8 * g + 4 * half);
+                    const f32x4 x = *reinterpret_cast<const f32x4*>(v + 32 * u + 8 * g + 4 * half);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int e = 4 * g + i;
-                        s[e] = __builtin_amdgcn_exp2f(s[e] - l4[i]);
-                        dp[e] = s[e] * (dp[e] - d4[i]);
-                        if (CAP) dp[e] *= 1.f - th[e] * th[e];
-                    }
+                    for (int i = 0; i < 4; ++i) r[4 * g + i] = x[i];
                 }
+                return r;
+            };
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u) {
+                f32x16 s = CAP ? splat(0.f) : rows16(lc, u), th, le;
+                RowOps<D> f;
+                f.load(fr, qc, 32 * u);
+                PHASE();
+                s = f.times(kf, s);
+                f.load(fr, gc, 32 * u);
+                f32x16 dp = rows16(dc, u);
+                const f32x16 bias = read_bias<BIAS>(win, pl, at_t + 32 * u, half, lane_off);
+                if (BIAS) pl.next();
+                if (CAP) le = rows16(lc, u);
+                PHASE();
+                dp = f.times(vf, dp);
+                ColOps<D> gt, qt;
+                gt.load(fr, gc, 32 * u);
+                if (D <= 64) qt.load(fr, qc, 32 * u);
+                PHASE();
+                to_logits<BIAS, CAP>(s, th, a, bias);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    s[i] = __builtin_amdgcn_exp2f(CAP ? s[i] - le[i] : s[i]);
+                    dp[i] *= s[i];
+                    if (CAP) dp[i] *= 1.f - th[i] * th[i];
+                }
+                if (D > 64) qt.load(fr, qc, 32 * u);
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
                     const bf16x8 pf = pack8(s, 8 * g), df = pack8(dp, 8 * g);
 #pragma unroll
                     for (int d = 0; d < DB; ++d) {
-                        dv[d] = mfma(fr.col(gc, 32 * u + 16 * g, d), pf, dv[d]);
-                        dk[d] = mfma(fr.col(qc, 32 * u + 16 * g, d), df, dk[d]);
+                        dv[d] = mfma(gt.f[g][d], pf, dv[d]);
+                        dk[d] = mfma(qt.f[g][d], df, dk[d]);
                     }
                 }
             }
-            if (t + 1 < nt) store(t + 1);
+            if (n + 1 < n_all) store(P ^ 1);
+        };
+        for (int n = 0; n < n_all; n += 2) {
+            tile(n, std::integral_constant<int, 0>{});
+            if (n + 1 < n_all) tile(n + 1, std::integral_constant<int, 1>{});
         }
     }
     if (key >= a.Lk) return;
@@ -786,27 +944,21 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : 2) void attn_dkv_kernel(AttnArg
 }
 
 // ======================================================================================================= host side
-// Tiles of 64 streamed tokens whose bias window, next to 128 owned ones, fits WIN_FLOATS (0: not even one does).
-int span_of(int n, int rows, int cols) {                              // the most P(last) - P(first) can be over n consecutive tokens
-    if (n <= 1) return 0;
-    int64_t crossings = rows > 1 ? (n - 2 + cols) / cols : 0;
-    if (crossings > rows - 1) crossings = rows - 1;
-    const int64_t s = (n - 1) + crossings * (cols - 1);
-    return s > (1 << 30) ? 1 << 30 : (int)s;
+// The bias window of a segment of `tiles` streamed tiles next to 128 owned rows, and (irregular grids) the table of its places.
+int64_t span_of(int64_t n, int rows, int cols) {                      // the most P(last) - P(first) can be over n consecutive tokens
+    return n <= 1 ? 0 : (n - 1) + (rows > 1 ? (n - 2 + cols) / cols * (cols - 1) : 0);
 }
-int segment_tiles(int owned, int streamed, int rows, int cols, int floats = WIN_FLOATS) {
-    const int own = span_of(owned < BLK ? owned : BLK, rows, cols);
-    const int tiles = ceil_div(streamed, KT);
-    int lo = 0;
-    for (int t = tiles; t > 0; t = t > 64 ? t / 2 : t - 1) {
-        const int64_t n = (int64_t)t * KT < streamed ? (int64_t)t * KT : streamed;
-        if ((int64_t)own + span_of((int)n, rows, cols) + 1 <= floats) { lo = t; break; }
+struct Window { int tiles, win_bytes; size_t lds; };
+// As many tiles as `budget` bytes hold; tiles 0: not even one.
+Window window_of(int bias, int owned, int streamed, int rows, int cols, int KT, int budget) {
+    Window w{};
+    if (bias == 0 || streamed == 0) return w;
+    for (int t = ceil_div(streamed, KT); t > 0; t = t > 64 ? t / 2 : t - 1) {
+        const int64_t win = 4 * (span_of(owned < BLK ? owned : BLK, rows, cols) + span_of((int64_t)t * KT, rows, cols) + 1 + WIN_PAD);
+        const int64_t all = (win + 15) / 16 * 16 + (bias == 1 ? 4 * (int64_t)t * KT : 0);
+        if (all <= budget) { w.tiles = t; w.win_bytes = (int)((win + 15) / 16 * 16); w.lds = (size_t)all; break; }
     }
-    return lo;
-}
-size_t window_bytes(int owned, int streamed, int rows, int cols, int seg) {
-    const int64_t n = (int64_t)seg * KT < streamed ? (int64_t)seg * KT : streamed;
-    return 4 * ((size_t)span_of(owned < BLK ? owned : BLK, rows, cols) + span_of((int)n, rows, cols) + 1 + WIN_PAD);
+    return w;
 }
 
 int check_desc(const rgbd_attn_desc* d, const char* who) {
@@ -819,6 +971,7 @@ int check_desc(const rgbd_attn_desc* d, const char* who) {
     RGBD_REQUIRE(d->cap >= 0.f, "%s: cap must not be negative", who);
     const int64_t st[9] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh};
     for (int i = 0; i < 9; ++i) RGBD_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
+    for (int i = 1; i < 9; i += 3) RGBD_REQUIRE(st[i] >= 0 && st[i] < (1 << 24), "%s: token strides must lie in [0, 2^24) elements", who);
     RGBD_REQUIRE((((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v) & 15) == 0, "%s: q, k, v must be 16-byte aligned", who);
     if (d->table) {
         RGBD_REQUIRE(d->map != nullptr && d->n_buckets > 0, "%s: a bias table needs its bucket map", who);
@@ -839,17 +992,19 @@ AttnArgs args_of(const rgbd_attn_desc* d) {
     a.table = d->table; a.map = d->map; a.lengths = d->lengths;
     a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.rep = d->H / d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk;
     a.rows = d->table ? d->rows : 1; a.cols = d->table ? d->cols : 1 << 24; a.q_start = d->table ? d->q_start : 0;
-    a.n_buckets = d->n_buckets;
+    a.pos_cols = a.rows > 1 ? a.cols : 1 << 30; a.n_buckets = d->n_buckets;
     a.scale = d->scale; a.cap = d->cap;
-    a.n_qb = ceil_div(d->Lq, BLK); a.n_kb = ceil_div(d->Lk, BLK); a.n_kt = ceil_div(d->Lk, KT);
+    a.n_qb = ceil_div(d->Lq, BLK); a.n_kb = ceil_div(d->Lk, BLK); a.kt = kt_of(d->D); a.n_kt = ceil_div(d->Lk, a.kt);
     a.lse = d->lse;
     return a;
 }
 
-// 0 no bias; 2 four aligned tokens of a streamed tile share a grid row; 1 they may not.
+// 0 no bias; 2 regular, 1 irregular grid (struct Places) for streamed tokens that begin at `first`.
 int bias_mode(const rgbd_attn_desc* d, int first) {
     if (!d->table) return 0;
-    return d->rows == 1 || (d->cols % 4 == 0 && first % 4 == 0) ? 2 : 1;
+    const bool wide = d->rows == 1 || (d->cols % 32 == 0 && first % 32 == 0);
+    const bool narrow = (d->cols == 4 || d->cols == 8 || d->cols == 16) && first % d->cols == 0;
+    return wide || narrow ? 2 : 1;
 }
 
 #define BY_BIAS_CAP(KERNEL, D, ...)                                                                                     \
@@ -898,12 +1053,12 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};
     z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
     if (!dt || d->Lq == 0 || d->Lk == 0) return z;
-    const int n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
+    const int KT = kt_of(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
         z.mode = DT_BLOCKS;
-        z.part = (int64_t)d->B * d->H * n_qb * 4 * n_kt * 2 * 64;
+        z.part = (int64_t)d->B * d->H * n_qb * 4 * n_kt * (KT / 32) * 64;
         z.gq = d->rows == 1 ? n_qb * 4 : d->cols / 32;
-        z.gk = d->rows == 1 ? n_kt * 2 : d->cols / 32;
+        z.gk = d->rows == 1 ? n_kt * (KT / 32) : d->cols / 32;
         z.q_row0 = d->rows == 1 ? 0 : d->q_start / d->cols;
         z.q_rows = d->rows == 1 ? 1 : ceil_div(d->Lq, d->cols);
         z.k_rows = d->rows == 1 ? 1 : ceil_div(d->Lk, d->cols);
@@ -930,12 +1085,11 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
     a.out = (unsigned short*)o;
     a.out_lo = (unsigned short*)o_lo;
     const int bias = bias_mode(d, 0);
-    size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4;
-    if (bias && d->Lk > 0) {
-        a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols);
-        RGBD_REQUIRE(a.seg_tiles > 0, "rgbd_attention_fwd: the bias of one tile does not fit (%d x %d grid)", a.rows, a.cols);
-        lds += window_bytes(d->Lq, d->Lk, a.rows, a.cols, a.seg_tiles);
-    }
+    const Window w = window_of(bias, d->Lq, d->Lk, a.rows, a.cols, a.kt, WIN_FWD);
+    RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "rgbd_attention_fwd: the bias of one tile does not fit (%d x %d grid)", a.rows, a.cols);
+    a.seg_tiles = w.tiles;
+    a.win_bytes = w.win_bytes;
+    const size_t lds = 4 * a.kt * 2 * d->D + w.lds;
     const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
     hipStream_t s = (hipStream_t)stream;
     const bool cap = d->cap > 0.f;
@@ -989,14 +1143,11 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
 
     if (d->Lq > 0) {
         const int bias = bias_mode(d, 0);
-        size_t lds = 4 * KT * 2 * d->D + 2 * KT * 4 + DT_LDS[z.mode];
-        a.seg_tiles = 1;
-        if (bias && d->Lk > 0) {
-            // with the table's gradient a workgroup keeps to half of the compute unit's LDS where the head size lets it
-            a.seg_tiles = segment_tiles(d->Lq, d->Lk, a.rows, a.cols, z.mode ? 2304 : WIN_FLOATS);
-            RGBD_REQUIRE(a.seg_tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
-            lds += window_bytes(d->Lq, d->Lk, a.rows, a.cols, a.seg_tiles);
-        }
+        const Window w = window_of(bias, d->Lq, d->Lk, a.rows, a.cols, a.kt, z.mode ? WIN_DQ : WIN_FWD);
+        RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
+        a.seg_tiles = w.tiles;
+        a.win_bytes = w.win_bytes;
+        const size_t lds = 4 * a.kt * 2 * d->D + dt_lds(z.mode, d->D) + w.lds;
         const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
         const int rc = d->D == 32 ? launch_dq<32>(a, bias, cap, z.mode, grid, lds, s) : d->D == 64 ? launch_dq<64>(a, bias, cap, z.mode, grid, lds, s)
                                                                                                : launch_dq<128>(a, bias, cap, z.mode, grid, lds, s);
@@ -1015,13 +1166,11 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
     if (z.mode) RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
     if (d->Lk > 0) {
         const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
-        size_t lds = 4 * KT * 2 * d->D + 6 * KT * 4;
-        a.seg_tiles = 1;
-        if (bias) {
-            a.seg_tiles = segment_tiles(d->Lk, d->Lq, a.rows, a.cols);
-            RGBD_REQUIRE(a.seg_tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
-            lds += window_bytes(d->Lk, d->Lq, a.rows, a.cols, a.seg_tiles);
-        }
+        const Window w = window_of(bias, d->Lk, d->Lq, a.rows, a.cols, a.kt, WIN_FWD);
+        RGBD_REQUIRE(bias == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
+        a.seg_tiles = w.tiles;
+        a.win_bytes = w.win_bytes;
+        const size_t lds = 4 * a.kt * 2 * d->D + 4 * a.kt * 4 + w.lds;
         const unsigned grid = (unsigned)a.B * a.Hkv * a.n_kb;
         const int rc = d->D == 32 ? launch_dkv<32>(a, bias, cap, grid, lds, s) : d->D == 64 ? launch_dkv<64>(a, bias, cap, grid, lds, s)
                                                                                             : launch_dkv<128>(a, bias, cap, grid, lds, s);
