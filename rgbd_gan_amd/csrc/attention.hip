@@ -700,14 +700,28 @@ __global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float
     const int dgs = gq + gk - 1;
     const int dy = cls / dgs - (k_rows - 1), dg = cls % dgs - (gk - 1);       // query group row (from q_row0) - key row, group - group
     const int y0 = max(0, dy), y1 = min(q_rows, k_rows + dy), g0 = max(0, dg), g1 = min(gq, gk + dg);
-    const int ny = max(0, y1 - y0), ng = max(0, g1 - g0), n = a.B * ny * ng;
     const int n_qg = a.n_qb * 4, n_kg = a.n_kt * (a.kt / 32);
+    // runs of blocks one step apart (down the rows; along the groups where there is one row), eight at a time, dealt out over the waves
+    const bool line = q_rows == 1 && k_rows == 1;
+    const int lo = line ? g0 : y0, hi_all = line ? g1 : y1, outer = line ? 1 : max(0, g1 - g0);
+    const int chunks = max(0, hi_all - lo + 7) / 8, tasks = a.B * outer * chunks;
+    const int64_t step = 64 * (line ? (int64_t)n_kg + 1 : (int64_t)gq * n_kg + gk);
+    const float* src = a.part + (int64_t)h * n_qg * n_kg * 64 + lane;
     float s = 0.f;
-    for (int e = r; e < n; e += 16) {
-        const int g = g0 + e % ng, y = y0 + e / ng % ny, b = e / (ng * ny);
-        const int qg = y * gq + g, kg = (y - dy) * gk + g - dg;
-        if (qg >= n_qg || kg >= a.kt / 32 * ((keys_of(a, b) + a.kt - 1) / a.kt)) continue;
-        s += a.part[((int64_t)((b * a.H + h) * n_qg + qg) * n_kg + kg) * 64 + lane];
+    for (int task = __builtin_amdgcn_readfirstlane(r); task < tasks; task += 16) {
+        const int o = task / chunks, first = lo + task % chunks * 8, b = o / outer, g = line ? 0 : g0 + o % outer;
+        const int k_valid = a.kt / 32 * ((keys_of(a, b) + a.kt - 1) / a.kt);      // key groups that were stored
+        // last block of the run: a query group that exists, a key group that was stored
+        const int hi = line ? min(hi_all, min(n_qg, k_valid + dg))
+                            : min(hi_all, min((n_qg - g + gq - 1) / gq, dy + (k_valid - (g - dg) + gk - 1) / gk));
+        if (first >= hi) continue;
+        const float* p = src + ((int64_t)b * a.H * n_qg + (line ? first : first * gq + g)) * n_kg * 64 +
+                         64 * (int64_t)(line ? first - dg : (first - dy) * gk + g - dg);
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p[min(j, hi - 1 - first) * step];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += first + j < hi ? v[j] : 0.f;
     }
     red[threadIdx.x] = s;
     __syncthreads();
