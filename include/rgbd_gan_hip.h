@@ -632,8 +632,10 @@ typedef struct {
     const int32_t* order;
     const int32_t* start;
 } rgbd_attn_grad;
-int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, void* stream);
-int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table);                 /* floats; -1: bad sizes */
+/* workspaces: floats, uninitialised (0: may be NULL; -1: bad sizes) */
+int64_t rgbd_attention_fwd_workspace(const rgbd_attn_desc* d);
+int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, float* workspace, void* stream);
+int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table);
 int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream);
 
 #ifdef __cplusplus

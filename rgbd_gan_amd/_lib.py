@@ -126,7 +126,8 @@ PROTOTYPES = {
     "rgbd_group_norm_workspace": ([c_int, c_int, c_int, c_int, c_int, c_int], c_int64),
     "rgbd_group_norm_fwd": ([_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float, _P], c_int),
     "rgbd_group_norm_bwd": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P], c_int),
-    "rgbd_attention_fwd": ([_P, _P, _P, _P], c_int),
+    "rgbd_attention_fwd_workspace": ([_P], c_int64),
+    "rgbd_attention_fwd": ([_P, _P, _P, _P, _P], c_int),
     "rgbd_attention_bwd_workspace": ([_P, c_int], c_int64),
     "rgbd_attention_bwd": ([_P, _P, _P, _P], c_int),
 }

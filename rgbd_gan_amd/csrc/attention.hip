@@ -39,7 +39,7 @@ struct AttnArgs {
     int64_t dq_sb, dq_sl, dq_sh, dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
     int B, H, Hkv, rep, Lq, Lk;
     int rows, cols, pos_cols, q_start, n_buckets;
-    int kt, n_qb, n_kb, n_kt, seg_tiles, win_bytes;
+    int kt, n_qb, n_kb, n_kt, seg_tiles, win_bytes, splits;
     int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
     float scale, cap;
 };
@@ -491,6 +491,213 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
         }
 }
 
+// ======================================================================================================= forward, few rows
+// At most 32 (query, head) pairs share a key / value head: all of them are the lanes of ONE product, so keys and values are read once
+// however many heads share them, and the keys are cut into `splits` runs for as many workgroups.  Bound by reading keys and values: a
+// wave streams blocks of 32 keys of its own (two buffers, no barrier in the loop), and the waves', then the runs', (maximum, sum,
+// output) are joined in a fixed order.  part: (B, Hkv, splits, 32, D + 2) fp32: output, maximum, sum.
+// LDS: for each wave K[2] V[2] of 32 rows; the joining reuses it.
+template <int D> struct WaveDma {
+    static constexpr int NP = D / 16;                                // 1 KB pieces of a block
+    unsigned lds;
+    __device__ __forceinline__ void init(const char* block) { lds = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)block; }
+    // rows k0 .. k0 + 31 (the last valid one repeated) into the block `bytes` behind
+    __device__ __forceinline__ void load(const unsigned short* p, int64_t sl, int k0, int valid, int bytes) const {
+        constexpr int RP = 512 / D, CH = D / 8;                       // rows of a piece, chunks of a row
+        const int lane = threadIdx.x & 63, r0 = lane / CH, ch = lane % CH;
+        const unsigned to = (unsigned)__builtin_amdgcn_readfirstlane((int)lds) + bytes;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int row = i * RP + r0;
+            const unsigned short* src = p + (int64_t)min(k0 + row, valid - 1) * sl + ((ch ^ swz<D>(row)) << 3);
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(to + 1024 * i), "v"(src) : "memory", "m0");
+        }
+    }
+};
+
+template <int D, bool BIAS, bool CAP>
+__global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int BB = 32 * 2 * D, KS = D / 16, DB = D / 32;          // bytes of a block
+    const int split = blockIdx.x % a.splits, bk = blockIdx.x / a.splits, hk = bk % a.Hkv, b = bk / a.Hkv;
+    const int lane = threadIdx.x & 63, wave = wave_id(), half = lane >> 5, col = lane & 31;
+    const int cols = a.rep * a.Lq;
+    const int h = hk * a.rep + min(col, cols - 1) / a.Lq, qi = min(col, cols - 1) % a.Lq;
+    const Frags<D> fr(lane);
+    char* mine = smem + wave * 4 * BB;
+    WaveDma<D> dma;
+    dma.init(mine);
+
+    const int len = keys_of(a, b), blocks = (len + 31) / 32;
+    const int per = (blocks + a.splits - 1) / a.splits, b1 = min(blocks, (split + 1) * per);
+    const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
+    const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
+
+    // the bias of a lane's 16 (pair, key): places first, then their buckets, one block ahead
+    const int pq = BIAS ? pos_of(a.q_start + qi, a.pos_cols) + (2 * a.cols - 1) * (a.rows - 1) + a.cols - 1 : 0;
+    const int last = (2 * a.cols - 1) * (2 * a.rows - 1) - 1;
+    const float* trow = BIAS ? a.table + (int64_t)h * a.n_buckets : nullptr;
+    const float inv_cols = BIAS ? 1.f / (float)a.pos_cols : 0.f;
+    int u[16];
+    float bias[16];
+    auto places = [&](int blk) {
+        const int x0 = blk * 32 % a.pos_cols, base = pq - pos_of(blk * 32, a.pos_cols);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int off = 8 * (i >> 2) + 4 * half + (i & 3);
+            // rows of the grid that off keys further on have ended: (x0 + off) / cols, a quotient below 2^12 at least 1 / 2048 off an integer
+            const int wraps = a.rows > 1 ? (int)(((float)(x0 + off) + 0.5f) * inv_cols) : 0;
+            u[i] = a.map[min(max(base - off - wraps * (a.cols - 1), 0), last)];
+        }
+    };
+    auto buckets = [&] {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) bias[i] = trow[min(max(u[i], 0), a.n_buckets - 1)] * LOG2E;
+    };
+
+    bf16x8 qf[KS];
+    {
+        const unsigned short* qp = a.q + b * a.q_sb + (int64_t)qi * a.q_sl + h * a.q_sh + 8 * half;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+    }
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = splat(0.f);
+    float m = NEG_INF, l = 0.f;
+    int blk = split * per + wave, p = 0;
+    if (blk < b1) {
+        dma.load(kp, a.k_sl, blk * 32, len, 0);
+        dma.load(vp, a.v_sl, blk * 32, len, 2 * BB);
+        if (BIAS) { places(blk); buckets(); }
+    }
+    arrived(qf);
+    for (; blk < b1; blk += 4, p ^= 1) {
+        float now[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) now[i] = BIAS ? bias[i] : 0.f;
+        dma_wait();
+        const bool more = blk + 4 < b1;
+        if (more) {
+            dma.load(kp, a.k_sl, (blk + 4) * 32, len, (p ^ 1) * BB);
+            dma.load(vp, a.v_sl, (blk + 4) * 32, len, (2 + (p ^ 1)) * BB);
+            if (BIAS) places(blk + 4);
+        }
+        RowOps<D> kf;
+        kf.load(fr, mine + p * BB, 0);
+        f32x16 x = kf.times(qf, splat(0.f)), th;
+        if (CAP) {
+            th = x;
+            tanh16(th, a.scale / a.cap);
+        }
+        const float f = CAP ? a.cap * LOG2E : a.scale * LOG2E;
+        float top = NEG_INF;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = (CAP ? th[i] : x[i]) * f + now[i];
+            if (blk * 32 + 8 * (i >> 2) + 4 * half + (i & 3) >= len) x[i] = NEG_INF;
+            top = fmaxf(top, x[i]);
+        }
+        top = other_half_max(top);
+        const float mn = fmaxf(m, top), ms = mn == NEG_INF ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        l *= al;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= al;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            x[i] = __builtin_amdgcn_exp2f(x[i] - ms);
+            l += x[i];
+        }
+        ColOps<D> vf;
+        vf.load(fr, mine + (2 + p) * BB, 0);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {                                // two bf16 terms of p: the matrix cores have time to spare here
+            const bf16x8 pf = pack8(x, 8 * g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[8 * g + i] -= (float)pf[i];
+            const bf16x8 pl = pack8(x, 8 * g);
+#pragma unroll
+            for (int d = 0; d < DB; ++d) {
+                o[d] = mfma(vf.f[g][d], pf, o[d]);
+                o[d] = mfma(vf.f[g][d], pl, o[d]);
+            }
+        }
+        if (BIAS && more) buckets();
+    }
+    l = other_half_sum(l);
+    // join the waves: (32, D) outputs and 32 (maximum, sum) of each
+    __syncthreads();
+    float* jo = reinterpret_cast<float*>(smem);                      // (4, 32, D + 1): a lane's column apart from its neighbour's
+    float* jm = jo + 4 * 32 * (D + 1);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) jo[(wave * 32 + col) * (D + 1) + 32 * d + 8 * (i >> 2) + 4 * half + (i & 3)] = o[d][i];
+    if (half == 0) { jm[wave * 64 + col] = m; jm[wave * 64 + 32 + col] = l; }
+    __syncthreads();
+    float* part = a.part + (int64_t)blockIdx.x * 32 * (D + 2);
+    for (int e = threadIdx.x; e < cols * D; e += 256) {
+        const int c = e / D, d = e % D;
+        float mm = NEG_INF, s = 0.f, ll = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, jm[w * 64 + c]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float al = __builtin_amdgcn_exp2f(jm[w * 64 + c] - (mm == NEG_INF ? 0.f : mm));
+            s += jo[(w * 32 + c) * (D + 1) + d] * al;
+            ll += jm[w * 64 + 32 + c] * al;
+        }
+        part[c * (D + 2) + d] = s;
+        if (d == 0) { part[c * (D + 2) + D] = mm; part[c * (D + 2) + D + 1] = ll; }
+    }
+}
+
+// A workgroup a (sample, query, head): the runs' partials joined, eight at a time by each of its 512 / D rows of D threads.
+constexpr int MAX_SPLITS = 512;
+template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(AttnArgs a) {
+    __shared__ float al[MAX_SPLITS], red[512];
+    const int d = threadIdx.x % D, r = threadIdx.x / D, h = blockIdx.x % a.H, qi = blockIdx.x / a.H % a.Lq, b = blockIdx.x / a.H / a.Lq;
+    const int hk = h / a.rep, c = h % a.rep * a.Lq + qi;
+    const float* part = a.part + (((int64_t)b * a.Hkv + hk) * a.splits * 32 + c) * (D + 2);
+    constexpr int64_t RUN = 32 * (D + 2);
+    constexpr int R = 512 / D;
+    // wave 0: every run's maximum and sum -> its factor, the row's maximum and sum
+    __shared__ float row_m, row_l;
+    if (threadIdx.x < 64) {
+        float mm = NEG_INF, ll = 0.f;
+        for (int i = threadIdx.x; i < a.splits; i += 64) { al[i] = part[i * RUN + D]; mm = fmaxf(mm, al[i]); }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+        for (int i = threadIdx.x; i < a.splits; i += 64) {
+            al[i] = __builtin_amdgcn_exp2f(al[i] - (mm == NEG_INF ? 0.f : mm));
+            ll += part[i * RUN + D + 1] * al[i];
+        }
+        ll = wave_sum(ll);
+        if (threadIdx.x == 0) { row_m = mm; row_l = ll; }
+    }
+    __syncthreads();
+    float s = 0.f;
+    for (int i0 = r; i0 < a.splits; i0 += R * 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = part[min(i0 + j * R, a.splits - 1) * RUN + d];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += i0 + j * R < a.splits ? v[j] * al[min(i0 + j * R, MAX_SPLITS - 1)] : 0.f;
+    }
+    red[threadIdx.x] = s;
+    __syncthreads();
+    if (r) return;
+    for (int k = 1; k < R; ++k) s += red[k * D + d];
+    const float l = row_l, y = l > 0.f ? s / l : (l == 0.f ? 0.f : l);
+    const int64_t at = (int64_t)blockIdx.x * D + d;
+    a.out[at] = f32_to_bf16_bits(y);
+    if (a.out_lo) a.out_lo[at] = f32_to_bf16_bits(y - bf16_bits_to_f32(f32_to_bf16_bits(y)));
+    if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + qi] = l == 0.f ? 0.f : row_m + __builtin_amdgcn_logf(l);
+}
+
 // ======================================================================================================= dq, delta and the table
 // Partials of the table's gradient, without global atomics and in one order of summation.  DT names how a 128 x 64 tile of ds (fp32,
 // never rounded) is reduced to sums over pairs of equal offset:
@@ -797,7 +1004,8 @@ __global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const
 
 // ======================================================================================================= dk, dv
 // A workgroup owns 128 keys of one key / value head and streams the queries of every head that shares it: scores here are
-// queries x keys, a lane holds one key.  No sum leaves the workgroup.
+// queries x keys, a lane holds one key.  No sum leaves the workgroup; where keys and heads alone are too few workgroups for the chip,
+// the tiles of queries are cut into `splits` runs whose fp32 sums a second launch adds up: part (splits, B, Hkv, Lk, 2 D).
 // LDS: Q[2] dO[2] | lse[2][64] | delta[2][64] | window | table of the segment's places (BIAS 1).
 template <int D, int BIAS, bool CAP>
 __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {
@@ -809,7 +1017,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
     int* at = reinterpret_cast<int*>(win + a.win_bytes);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
-    const int kb = id % a.n_kb, bk = id / a.n_kb, hk = bk % a.Hkv, b = bk / a.Hkv;
+    const int split = id % a.splits, kb = id / a.splits % a.n_kb, bk = id / a.splits / a.n_kb, hk = bk % a.Hkv, b = bk / a.Hkv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int key = kb * BLK + wave * 32 + (lane & 31);
     const Frags<D> fr(lane);
@@ -839,10 +1047,10 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
 
         Dma<D> sq, sg;
         float next_l = 0.f, next_d = 0.f;
-        auto load = [&](int h, int t, int buf) {                      // tile t of head h into buffer buf
-            if (t == 0) {
-                sq.init(a.q + b * a.q_sb + h * a.q_sh, a.q_sl, a.Lq, smem);
-                sg.init(a.d_o + ((int64_t)b * a.Lq * a.H + h) * D, (int64_t)a.H * D, a.Lq, smem + 2 * TB);
+        auto load = [&](int h, int t, int buf, bool first) {          // tile t of head h into buffer buf
+            if (t == 0 || first) {
+                sq.init(a.q + b * a.q_sb + h * a.q_sh + (int64_t)t * KT * a.q_sl, a.q_sl, a.Lq - t * KT, smem);
+                sg.init(a.d_o + (((int64_t)b * a.Lq + t * KT) * a.H + h) * D, (int64_t)a.H * D, a.Lq - t * KT, smem + 2 * TB);
             }
             sq.next(a.q_sl, buf * TB);
             sg.next((int64_t)a.H * D, buf * TB);
@@ -861,21 +1069,23 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
             dma_wait();
         };
         Places<BIAS> pl;
-        int h = hk * a.rep, t = 0, seg_t = 0;                        // the tile at hand: head, tile of its queries
-        load(h, 0, 0);
-        store(0);
+        const int n_all = nqt * a.rep, per = (n_all + a.splits - 1) / a.splits, n0 = split * per, n1 = min(n_all, n0 + per);
+        int h = hk * a.rep + n0 / nqt, t = n0 % nqt, seg_t = 0;      // the tile at hand: head, tile of its queries
+        if (n0 < n1) {
+            load(h, t, 0, true);
+            store(0);
+        }
         arrived(kf);
         arrived(vf);
-        const int n_all = nqt * a.rep;
         auto tile = [&](int n, auto parity) {
             constexpr int P = decltype(parity)::value;
             const char* qc = smem + P * TB;
             const char* gc = smem + (2 + P) * TB;
             const float* lc = ls + P * KT;
             const float* dc = dl + P * KT;
-            if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
+            if (BIAS && (n == n0 || t == 0 || t == seg_t + a.seg_tiles)) {
                 __syncthreads();
-                if (t == 0) pl.init(a, a.q_start);
+                if (n == n0 || t == 0) pl.init(a, a.q_start + t * KT);
                 seg_t = t;
                 pl.blk = 0;
                 const int rows = a.seg_tiles * KT, first = a.q_start + t * KT, p0 = pos_of(first, a.pos_cols);
@@ -885,7 +1095,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
             __syncthreads();
             const int* at_t = at + (t - seg_t) * KT;
             if (++t == nqt) { t = 0; ++h; }
-            if (n + 1 < n_all) load(h, t, P ^ 1);
+            if (n + 1 < n1) load(h, t, P ^ 1, false);
             PHASE();
             auto rows16 = [&](const float* v, int u) {                // a value per streamed row of the block, as the products lie
                 f32x16 r;
@@ -933,15 +1143,27 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
                     }
                 }
             }
-            if (n + 1 < n_all) store(P ^ 1);
+            if (n + 1 < n1) store(P ^ 1);
         };
-        for (int n = 0; n < n_all; n += 2) {
+        for (int n = n0; n < n1; n += 2) {
             tile(n, std::integral_constant<int, 0>{});
-            if (n + 1 < n_all) tile(n + 1, std::integral_constant<int, 1>{});
+            if (n + 1 < n1) tile(n + 1, std::integral_constant<int, 1>{});
         }
     }
     if (key >= a.Lk) return;
     const bool in = key < len;
+    if (a.splits > 1) {                                              // (keys beyond the length: attn_kv_sum_kernel does not read them)
+        if (!in) return;
+        float* p = a.part + (((int64_t)split * a.B * a.Hkv + bk) * a.Lk + key) * 2 * D + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                *reinterpret_cast<f32x4*>(p + 32 * d + 8 * g) = f32x4{dk[d][4 * g], dk[d][4 * g + 1], dk[d][4 * g + 2], dk[d][4 * g + 3]};
+                *reinterpret_cast<f32x4*>(p + D + 32 * d + 8 * g) = f32x4{dv[d][4 * g], dv[d][4 * g + 1], dv[d][4 * g + 2], dv[d][4 * g + 3]};
+            }
+        return;
+    }
     unsigned short* ko = a.dk + b * a.dk_sb + (int64_t)key * a.dk_sl + hk * a.dk_sh + 4 * half;
     unsigned short* vo = a.dv + b * a.dv_sb + (int64_t)key * a.dv_sl + hk * a.dv_sh + 4 * half;
 #pragma unroll
@@ -955,6 +1177,34 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
             *reinterpret_cast<u32x2*>(ko + 32 * d + 8 * g) = w;
             *reinterpret_cast<u32x2*>(vo + 32 * d + 8 * g) = x;
         }
+}
+
+// dk, dv from the runs' sums: four values a thread, grid (tokens x heads x 2 D / 4 / 256).
+__global__ __launch_bounds__(256) void attn_kv_sum_kernel(AttnArgs a, int D) {
+    const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x, per = D / 2;           // groups of four a (sample, head, key)
+    const int64_t row = e / per, total = (int64_t)a.B * a.Hkv * a.Lk;
+    if (row >= total) return;
+    const int c = (int)(e % per) * 4, key = (int)(row % a.Lk), hk = (int)(row / a.Lk % a.Hkv), b = (int)(row / a.Lk / a.Hkv);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (key < keys_of(a, b)) {
+        const float* p = a.part + row * 2 * D + c;
+        const int64_t run = total * 2 * D;
+        for (int i0 = 0; i0 < a.splits; i0 += 4) {
+            f32x4 v[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(p + min(i0 + j, a.splits - 1) * run);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (i0 + j < a.splits)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) s[k] += v[j][k];
+        }
+    }
+    const bool is_k = c < D;
+    const float f = is_k ? a.scale : 1.f;
+    unsigned short* o = is_k ? a.dk + b * a.dk_sb + (int64_t)key * a.dk_sl + hk * a.dk_sh + c
+                             : a.dv + b * a.dv_sb + (int64_t)key * a.dv_sl + hk * a.dv_sh + c - D;
+    *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16x2(s[0] * f, s[1] * f), pack_bf16x2(s[2] * f, s[3] * f)};
 }
 
 // ======================================================================================================= host side
@@ -1062,10 +1312,44 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
 }
 
 // Floats of the backward workspace: delta, the partials and what the first reduction leaves of them.
-struct BwdSizes { int64_t delta, part, sums; int mode, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
+// Few (query, head) pairs over many keys: the number of runs the keys are cut into, 0 for the other form.  Both read a key block once a
+// workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.
+int few_splits(const rgbd_attn_desc* d) {
+    if ((int64_t)d->H / d->Hkv * d->Lq > 32 || d->Lk <= 256) return 0;
+    const int64_t groups = (int64_t)d->B * d->Hkv, want = d->D == 128 ? 256 : 512;   // workgroups that fit the chip at once (LDS)
+    int64_t s = (want + groups - 1) / groups;
+    const int64_t most = ceil_div(d->Lk, 32 * 8);                     // two blocks for every wave
+    if (s > most) s = most;
+    if (s > MAX_SPLITS) s = MAX_SPLITS;
+    return (int)(s < 1 ? 1 : s);
+}
+template <int D> int launch_few(const AttnArgs& a, bool bias, bool cap, hipStream_t s) {
+    const unsigned grid = (unsigned)a.B * a.Hkv * a.splits;
+    const size_t lds = 4 * 4 * 32 * 2 * D > 4 * (4 * 32 * (D + 1) + 256) ? 4 * 4 * 32 * 2 * D : 4 * (4 * 32 * (D + 1) + 256);
+    if (bias) { if (cap) LAUNCH((attn_few_kernel<D, true, true>)); else LAUNCH((attn_few_kernel<D, true, false>)); }
+    else { if (cap) LAUNCH((attn_few_kernel<D, false, true>)); else LAUNCH((attn_few_kernel<D, false, false>)); }
+    hipLaunchKernelGGL((attn_few_join_kernel<D>), dim3(a.B * a.H * a.Lq), dim3(512), 0, s, a);
+    return 0;
+}
+
+// Runs of query tiles for dk, dv: as many as fill the chip once (one workgroup a compute unit at head size 128, two at 64, three at 32:
+// registers), of at least four tiles each.
+int kv_splits(const rgbd_attn_desc* d) {
+    const int64_t groups = (int64_t)d->B * d->Hkv * ceil_div(d->Lk, BLK), want = d->D == 128 ? 256 : d->D == 64 ? 512 : 768;
+    if (groups == 0 || groups * 4 > want * 3) return 1;
+    int64_t s = want / groups;
+    const int64_t most = (int64_t)d->H / d->Hkv * ceil_div(d->Lq, kt_of(d->D)) / 4;
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    return (int)(s < 1 ? 1 : s);
+}
+
+struct BwdSizes { int64_t delta, part, sums, kv; int mode, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
 BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};
     z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
+    const int ks = kv_splits(d);
+    z.kv = ks > 1 ? (int64_t)ks * d->B * d->Hkv * d->Lk * 2 * d->D : 0;
     if (!dt || d->Lq == 0 || d->Lk == 0) return z;
     const int KT = kt_of(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
@@ -1085,12 +1369,19 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
         z.n_dist = d->q_start + n_qb * BLK - z.d0;
         z.sums = (int64_t)d->H * 2 * z.n_dist;
     }
+    z.sums = (z.sums + 3) / 4 * 4;
     return z;
 }
 
 }  // namespace
 
-extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, void* stream) {
+extern "C" int64_t rgbd_attention_fwd_workspace(const rgbd_attn_desc* d) {
+    if (check_desc(d, "rgbd_attention_fwd_workspace")) return -1;
+    if (d->B == 0 || d->Lq == 0) return 0;
+    return (int64_t)d->B * d->Hkv * few_splits(d) * 32 * (d->D + 2);
+}
+
+extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, float* workspace, void* stream) {
     if (check_desc(d, "rgbd_attention_fwd")) return -1;
     if (d->B == 0 || d->Lq == 0) return 0;
     RGBD_REQUIRE(d->q && o && (d->Lk == 0 || (d->k && d->v)), "rgbd_attention_fwd: null pointer");
@@ -1098,6 +1389,17 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
     AttnArgs a = args_of(d);
     a.out = (unsigned short*)o;
     a.out_lo = (unsigned short*)o_lo;
+    const bool cap = d->cap > 0.f;
+    hipStream_t s = (hipStream_t)stream;
+    a.splits = few_splits(d);
+    if (a.splits) {
+        RGBD_REQUIRE(workspace != nullptr, "rgbd_attention_fwd: null workspace");
+        a.part = workspace;
+        const int rc = d->D == 32 ? launch_few<32>(a, d->table, cap, s) : d->D == 64 ? launch_few<64>(a, d->table, cap, s) : launch_few<128>(a, d->table, cap, s);
+        if (rc) return rc;
+        RGBD_CHECK_LAUNCH("rgbd_attention_fwd (few rows)");
+        return 0;
+    }
     const int bias = bias_mode(d, 0);
     const Window w = window_of(bias, d->Lq, d->Lk, a.rows, a.cols, a.kt, WIN_FWD);
     RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "rgbd_attention_fwd: the bias of one tile does not fit (%d x %d grid)", a.rows, a.cols);
@@ -1105,8 +1407,6 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
     a.win_bytes = w.win_bytes;
     const size_t lds = 4 * a.kt * 2 * d->D + w.lds;
     const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
-    hipStream_t s = (hipStream_t)stream;
-    const bool cap = d->cap > 0.f;
     const bool fine = d->fine && bias;
     const int rc = d->D == 32   ? launch_fwd<32>(a, bias, cap, fine, grid, lds, s)
                    : d->D == 64 ? launch_fwd<64>(a, bias, cap, fine, grid, lds, s)
@@ -1119,7 +1419,7 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
 extern "C" int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table) {
     if (check_desc(d, "rgbd_attention_bwd_workspace")) return -1;
     const BwdSizes z = bwd_sizes(d, want_table && d->table);
-    return z.delta + z.part + z.sums + 4;
+    return z.delta + z.part + z.sums + z.kv + 4;
 }
 
 extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream) {
@@ -1185,10 +1485,14 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
         a.seg_tiles = w.tiles;
         a.win_bytes = w.win_bytes;
         const size_t lds = 4 * a.kt * 2 * d->D + 4 * a.kt * 4 + w.lds;
-        const unsigned grid = (unsigned)a.B * a.Hkv * a.n_kb;
+        a.splits = kv_splits(d);
+        a.part = workspace + z.delta + z.part + z.sums;
+        const unsigned grid = (unsigned)a.B * a.Hkv * a.n_kb * a.splits;
         const int rc = d->D == 32 ? launch_dkv<32>(a, bias, cap, grid, lds, s) : d->D == 64 ? launch_dkv<64>(a, bias, cap, grid, lds, s)
                                                                                             : launch_dkv<128>(a, bias, cap, grid, lds, s);
         if (rc) return rc;
+        if (a.splits > 1)
+            hipLaunchKernelGGL(attn_kv_sum_kernel, dim3((unsigned)(((int64_t)a.B * a.Hkv * a.Lk * (d->D / 2) + 255) / 256)), dim3(256), 0, s, a, d->D);
         RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dk, dv)");
     }
     return 0;

@@ -1703,9 +1703,14 @@ def attention_fwd(q, k, v, table=None, buckets=None, lengths=None, scale=None, c
         o_lo = torch.empty_like(o)
         lse = torch.empty(d.B, d.H, d.Lq, dtype=F32, device=q.device)
         d.lse = lse.data_ptr()
+    lib = _lib.load()
+    n = lib.rgbd_attention_fwd_workspace(ctypes.byref(d))
+    if n < 0:
+        _lib.check(-1, "rgbd_attention_fwd_workspace")
+    ws = torch.empty(n, dtype=F32, device=q.device) if n else None
     flops = 4 * d.B * d.H * d.Lq * d.Lk * d.D
-    rc = _timed("attn_fwd", flops, 4 * o.numel() + 4 * k.numel(), lambda: _lib.load().rgbd_attention_fwd(
-        ctypes.byref(d), _ptr(o), _ptr(o_lo), _stream()))
+    rc = _timed("attn_fwd", flops, 4 * o.numel() + 4 * k.numel(), lambda: lib.rgbd_attention_fwd(
+        ctypes.byref(d), _ptr(o), _ptr(o_lo), _ptr(ws), _stream()))
     _lib.check(rc, "rgbd_attention_fwd")
     return o, o_lo, lse
 

@@ -127,7 +127,7 @@ def test_c_entries_report_bad_arguments():
     assert lib.rgbd_group_norm_fwd(8, 16, 16, 16, 16, 16, 16, 2, 16, 2048, 4, 0, 0, 1e-5, 0.2, None) == -1
     assert b"channels" in lib.rgbd_last_error()
     assert lib.rgbd_group_norm_bwd(16, 8, 16, 16, 16, 16, 16, 16, 16, 16, 2, 16, 2048, 4, 0, 0, 0.2, None) == -1
-    assert lib.rgbd_attention_fwd(None, None, None, None) == -1
+    assert lib.rgbd_attention_fwd(None, None, None, None, None) == -1
     d = kernels._AttnDesc()
     d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D = 1, 2, 1, 4, 4, 64
     ok = lambda: lib.rgbd_attention_bwd_workspace(ctypes.byref(d), 0)
@@ -144,7 +144,7 @@ def test_c_entries_report_bad_arguments():
     assert ok() == -1 and b"outside" in lib.rgbd_last_error()
     d.cols = 4
     assert ok() > 0
-    assert lib.rgbd_attention_fwd(ctypes.byref(d), None, None, None) == -1 and b"null" in lib.rgbd_last_error()
+    assert lib.rgbd_attention_fwd(ctypes.byref(d), None, None, None, None) == -1 and b"null" in lib.rgbd_last_error()
     assert lib.rgbd_attention_bwd(ctypes.byref(d), None, None, None) == -1
     g = kernels._AttnGrad()
     assert lib.rgbd_attention_bwd(ctypes.byref(d), ctypes.byref(g), None, None) == -1 and b"null" in lib.rgbd_last_error()
