@@ -644,11 +644,11 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 extern "C" int64_t rgbd_group_norm_workspace(int B, int N, int C, int groups, int dtype, int backward) {
     if (gn_check(nullptr, B, N, C, groups, dtype, 0, "rgbd_group_norm_workspace")) return -1;
     // the vector and the scalar form cut a sample differently: room for either
-    int64_t most = 1;
+    int64_t most = backward ? 1 : 0;
     for (int al = 0; al < 2; ++al) {
         const GnPlan p = gn_plan(B, N, C, groups, dtype ? 4 : 2, al != 0, backward ? BWD_MOST : FWD_MOST);
         const int64_t f = backward ? (p.resident ? (int64_t)2 * B * C : (int64_t)2 * B * p.slabs * (C + groups))
-                                   : (p.resident ? 1 : (int64_t)2 * B * p.slabs * groups);
+                                   : (p.resident ? 0 : (int64_t)2 * B * p.slabs * groups);
         if (f > most) most = f;
     }
     return most;
@@ -659,10 +659,11 @@ extern "C" int rgbd_group_norm_fwd(const void* x, const float* gamma, const floa
                                    void* stream) {
     if (gn_check(x, B, N, C, groups, dtype, act, "rgbd_group_norm_fwd")) return -1;
     if (B == 0 || N == 0) return 0;
-    RGBD_REQUIRE(x && gamma && beta && y && mean && rstd && workspace, "rgbd_group_norm_fwd: null pointer");
+    RGBD_REQUIRE(x && gamma && beta && y && mean && rstd, "rgbd_group_norm_fwd: null pointer");
     RGBD_REQUIRE(eps >= 0.f, "rgbd_group_norm_fwd: eps must not be negative");
     const GnPlan p = gn_plan(B, N, C, groups, dtype ? 4 : 2, aligned16(x) && aligned16(y), FWD_MOST);
     RGBD_REQUIRE(p.pl > 0, "rgbd_group_norm_fwd: C=%d does not fit a workgroup", C);
+    RGBD_REQUIRE(p.resident || workspace, "rgbd_group_norm_fwd: null workspace");
     GnArgs a{};
     a.x = x; a.gamma = gamma; a.beta = beta; a.out = y; a.mean = mean; a.rstd = rstd; a.part = workspace;
     a.B = B; a.N = N; a.C = C; a.G = groups; a.cpg = C / groups; a.eps = eps; a.slope = slope;

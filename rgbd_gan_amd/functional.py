@@ -1674,23 +1674,25 @@ def fold_weight(W, mode, Cop, Cip):
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, groups, eps, act, slope):
-        y, mean, rstd = kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)
-        ctx.groups, ctx.act, ctx.slope = groups, act, slope
-        ctx.save_for_backward(x, gamma, beta, mean, rstd)
+        y, stats = kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)
+        ctx.spec = (groups, act, slope)
+        ctx.save_for_backward(x, gamma, beta, stats)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, gamma, beta, mean, rstd = ctx.saved_tensors
-        dx, dgamma, dbeta = kernels.group_norm_bwd(x, dy.contiguous(), gamma, beta, mean, rstd, ctx.groups, ctx.act, ctx.slope)
-        return dx, dgamma, dbeta, None, None, None, None
+        x, gamma, beta, stats = ctx.saved_tensors
+        return *kernels.group_norm_bwd(x, dy.contiguous(), gamma, beta, stats, *ctx.spec), None, None, None, None
 
 
 def group_norm(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
     """act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and variance over each sample's groups of C / groups neighbouring
     channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu"."""
-    return _GroupNorm.apply(x.contiguous(), gamma.contiguous(), beta.contiguous(), groups, eps, act, slope)
+    x, gamma, beta = x.contiguous(), gamma.contiguous(), beta.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
+        return _GroupNorm.apply(x, gamma, beta, groups, eps, act, slope)
+    return kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)[0]
 
 
 class RelativeBuckets:
@@ -1737,50 +1739,50 @@ class RelativeBuckets:
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, lengths, spec):
-        o, o_lo, lse = kernels.attention_fwd(q, k, v, table, lengths=lengths, keep=True, fine=ctx.needs_input_grad[3], **spec)
-        ctx.spec = spec
+    def forward(ctx, q, k, v, table, lengths, buckets, spec):
+        o, o_lo, lse = kernels.attention_fwd(kernels.AttnOperands.of(q, k, v), table, buckets, lengths, *spec, keep=True,
+                                             fine=ctx.needs_input_grad[3])
+        ctx.buckets, ctx.spec = buckets, spec
         ctx.save_for_backward(q, k, v, table, lengths, o, o_lo, lse)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
-        q, k, v, table, lengths, o, o_lo, lse = ctx.saved_tensors
-        dq, dk, dv, dtable = kernels.attention_bwd(q, k, v, d_o.contiguous(), o, o_lo, lse, table, lengths=lengths,
-                                                   want_table=ctx.needs_input_grad[3], **ctx.spec)
-        return dq, dk, dv, dtable, None, None
-
-
-def _packed_views(qkv, heads, kv_heads, D):
-    B, N, _ = qkv.shape
-    view = lambda lo, n: qkv[:, :, lo * D:(lo + n) * D].unflatten(2, (n, D))
-    return view(0, heads), view(heads, kv_heads), view(heads + kv_heads, kv_heads)
+        q, k, v, table, lengths, *kept = ctx.saved_tensors
+        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
+        of = kernels.AttnOperands.of
+        dtable = kernels.attention_bwd(of(q, k, v), of(*grads), d_o.contiguous(), *kept, table, ctx.buckets, lengths, *ctx.spec,
+                                       want_table=ctx.needs_input_grad[3])
+        return *grads, dtable, None, None, None
 
 
 class _AttentionPacked(torch.autograd.Function):
     """The three gradients are written into one tensor of the packed layout."""
 
     @staticmethod
-    def forward(ctx, qkv, table, lengths, layout, spec):
-        o, o_lo, lse = kernels.attention_fwd(*_packed_views(qkv, *layout), table, lengths=lengths, keep=True,
-                                            fine=ctx.needs_input_grad[1], **spec)
-        ctx.layout, ctx.spec = layout, spec
+    def forward(ctx, qkv, table, lengths, buckets, heads, spec):
+        o, o_lo, lse = kernels.attention_fwd(kernels.AttnOperands.packed(qkv, *heads), table, buckets, lengths, *spec, keep=True,
+                                             fine=ctx.needs_input_grad[1])
+        ctx.buckets, ctx.heads, ctx.spec = buckets, heads, spec
         ctx.save_for_backward(qkv, table, lengths, o, o_lo, lse)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
-        qkv, table, lengths, o, o_lo, lse = ctx.saved_tensors
+        qkv, table, lengths, *kept = ctx.saved_tensors
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
-        dtable = kernels.attention_bwd(*_packed_views(qkv, *ctx.layout), d_o.contiguous(), o, o_lo, lse, table, lengths=lengths,
-                                       out=_packed_views(dqkv, *ctx.layout), want_table=ctx.needs_input_grad[1], **ctx.spec)[3]
-        return dqkv, dtable, None, None, None
+        of = kernels.AttnOperands.packed
+        dtable = kernels.attention_bwd(of(qkv, *ctx.heads), of(dqkv, *ctx.heads), d_o.contiguous(), *kept, table, ctx.buckets, lengths,
+                                       *ctx.spec, want_table=ctx.needs_input_grad[1])
+        return dqkv, dtable, None, None, None, None
 
 
-def _attention_spec(buckets, scale, cap, q_start):
-    return dict(buckets=buckets, scale=scale, cap=float(cap or 0.0), q_start=int(q_start))
+def _readable(t):
+    """t, or a copy where the kernels cannot read it as it lies (kernels.AttnOperands refuses what is no tensor of theirs at all)."""
+    op = kernels.AttnOperands
+    return t if op.readable(t, op._axis(t, t.dim() - 1)) else t.clone(memory_format=torch.contiguous_format)
 
 
 def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=None, q_start=0):
@@ -1790,13 +1792,13 @@ def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=No
     head h // (H // Hkv)); scale defaults to D ** -0.5, cap 0 leaves scores uncapped; lengths (B,) int32 on the device.
     table (H, n_buckets) fp32 with `buckets` (RelativeBuckets): the bias table[h, bucket of the offset], query i at token
     q_start + i of the grid, key j at token j.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table."""
-    spec = _attention_spec(buckets, scale, cap, q_start)
-    q, k, v = (t if t.dim() != 4 or kernels.attention_readable(t) else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    spec = (None if scale is None else float(scale), float(cap or 0.0), int(q_start))
+    q, k, v = _readable(q), _readable(k), _readable(v)
     table = table.contiguous() if table is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, table)):
-        return _Attention.apply(q, k, v, table, lengths, spec)
-    return kernels.attention_fwd(q, k, v, table, lengths=lengths, **spec)[0]
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+        return _Attention.apply(q, k, v, table, lengths, buckets, spec)
+    return kernels.attention_fwd(kernels.AttnOperands.of(q, k, v), table, buckets, lengths, *spec)[0]
 
 
 def attention_packed(qkv, heads, kv_heads=None, table=None, buckets=None, scale=None, cap=0.0, lengths=None):
@@ -1807,12 +1809,10 @@ def attention_packed(qkv, heads, kv_heads=None, table=None, buckets=None, scale=
         qkv = qkv.flatten(1, 2)
     if qkv.dim() != 3 or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
         raise RuntimeError(f"attention_packed: {tuple(qkv.shape)} does not split into {heads} + 2 x {kv_heads} heads")
-    layout = (heads, kv_heads, qkv.shape[2] // (heads + 2 * kv_heads))
-    spec = _attention_spec(buckets, scale, cap, 0)
-    if not kernels.attention_readable(qkv.unsqueeze(2)):
-        qkv = qkv.clone(memory_format=torch.contiguous_format)
+    spec = (None if scale is None else float(scale), float(cap or 0.0), 0)
+    qkv = _readable(qkv)
     table = table.contiguous() if table is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
     if torch.is_grad_enabled() and (qkv.requires_grad or (table is not None and table.requires_grad)):
-        return _AttentionPacked.apply(qkv, table, lengths, layout, spec)
-    return kernels.attention_fwd(*_packed_views(qkv, *layout), table, lengths=lengths, **spec)[0]
+        return _AttentionPacked.apply(qkv, table, lengths, buckets, (heads, kv_heads), spec)
+    return kernels.attention_fwd(kernels.AttnOperands.packed(qkv, heads, kv_heads), table, buckets, lengths, *spec)[0]

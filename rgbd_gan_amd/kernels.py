@@ -1,6 +1,7 @@
 """Thin, typed wrappers: torch device tensors in, C-ABI calls out.  No arithmetic happens here."""
 import contextlib
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -1538,76 +1539,88 @@ def fold_weight(src, mode, Co, Ci, K, Cop, Cip, adjoint=False, out=None):
 
 
 # ------------------------------------------------------------------ group norm, attention
+# (their wrappers run once a layer on maps whose kernels take 10 us: no tensor or ctypes object is made that is not needed)
 ACTS = {None: 0, "none": 0, "lrelu": 1, "silu": 2}
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _chk_device(what, *tensors):
-    """Every tensor on the current device: the launch goes to that device's current stream."""
-    cur = torch.cuda.current_device()
+def _launch_stream(what, *tensors):
+    """The current device's current stream; every tensor must be on that device."""
+    cur = _current_device()
     for t in tensors:
-        if t is not None and t.device.index != cur:
+        if t is not None and t.get_device() != cur:
             raise RuntimeError(f"{what}: tensor on {t.device}, current device is cuda:{cur}")
+    return _raw_stream_of(cur)
 
 
 def _gn_sizes(x, gamma, beta, groups, act):
     if not torch.is_tensor(x) or x.dim() < 2:
         raise RuntimeError("group_norm: x must have a batch and a channel axis, (B, ..., C)")
-    if x.dtype not in (BF16, F32):
-        raise RuntimeError(f"group_norm: x must be bf16 or fp32, got {x.dtype}")
+    dt = x.dtype
+    if dt != BF16 and dt != F32:
+        raise RuntimeError(f"group_norm: x must be bf16 or fp32, got {dt}")
     if act not in ACTS:
         raise RuntimeError(f"group_norm: act must be one of {sorted(k for k in ACTS if k)}, got {act!r}")
-    C = x.shape[-1]
+    shape = x.shape
+    B, C = shape[0], shape[-1]
     groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise RuntimeError(f"group_norm: {groups} groups do not divide {C} channels")
-    for t, name in ((gamma, "gamma"), (beta, "beta")):
-        if tuple(t.shape) != (C,):
-            raise RuntimeError(f"group_norm: {name} must have shape ({C},), got {tuple(t.shape)}")
+    if gamma.shape != (C,):
+        raise RuntimeError(f"group_norm: gamma must have shape ({C},), got {tuple(gamma.shape)}")
+    if beta.shape != (C,):
+        raise RuntimeError(f"group_norm: beta must have shape ({C},), got {tuple(beta.shape)}")
     N = 1
-    for n in x.shape[1:-1]:
+    for n in shape[1:-1]:
         N *= n
-    _chk(x, x.dtype, "x"); _chk(gamma, F32, "gamma"); _chk(beta, F32, "beta")
-    _chk_device("group_norm", x, gamma, beta)
-    return x.shape[0], N, C, groups, 0 if x.dtype == BF16 else 1
+    _chk(x, dt, "x"); _chk(gamma, F32, "gamma"); _chk(beta, F32, "beta")
+    return B, N, C, groups, 0 if dt == BF16 else 1
 
 
-def _gn_workspace(sizes, backward, device):
-    n = _lib.load().rgbd_group_norm_workspace(*sizes, int(backward))
+@functools.lru_cache(maxsize=256)
+def _gn_workspace_floats(B, N, C, groups, dtype, backward):
+    n = _lib.load().rgbd_group_norm_workspace(B, N, C, groups, dtype, backward)
     if n < 0:
         _lib.check(-1, "rgbd_group_norm_workspace")
-    return torch.empty(n, dtype=F32, device=device)
+    return n
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
-    """x (B, ..., C) bf16 or fp32, gamma, beta (C,) fp32 -> y like x, mean, rstd (B, groups) fp32."""
-    B, N, C, groups, dt = sizes = _gn_sizes(x, gamma, beta, groups, act)
+    """x (B, ..., C) bf16 or fp32, gamma, beta (C,) fp32 -> y like x, stats (2, B, groups) fp32: the groups' means and 1 / sqrt(var + eps)."""
+    B, N, C, groups, dt = _gn_sizes(x, gamma, beta, groups, act)
     if not eps >= 0:
         raise RuntimeError(f"group_norm: eps must not be negative, got {eps}")
+    stream = _launch_stream("group_norm", x, gamma, beta)
     y = torch.empty_like(x)
-    stats = torch.empty(2, B, groups, dtype=F32, device=x.device)
-    ws = _gn_workspace(sizes, False, x.device)
+    n = _gn_workspace_floats(B, N, C, groups, dt, 0)
+    # statistics and workspace in one allocation
+    buf = torch.empty(2 * B * groups + n, dtype=F32, device=x.device)
+    p = buf.data_ptr()
     rc = _timed("gn_fwd", 0, 2 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_fwd(
-        _ptr(x), _ptr(gamma), _ptr(beta), _ptr(y), _ptr(stats[0]), _ptr(stats[1]), _ptr(ws), B, N, C, groups, dt, ACTS[act],
-        float(eps), float(slope), _stream()))
-    _lib.check(rc, "rgbd_group_norm_fwd")
-    return y, stats[0], stats[1]
+        x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), p, p + 4 * B * groups, p + 8 * B * groups, B, N, C, groups, dt,
+        ACTS[act], eps, slope, stream))
+    if rc:
+        _lib.check(rc, "rgbd_group_norm_fwd")
+    return y, buf if n == 0 else buf[:2 * B * groups]
 
 
-def group_norm_bwd(x, dy, gamma, beta, mean, rstd, groups, act=None, slope=0.2):
+def group_norm_bwd(x, dy, gamma, beta, stats, groups, act=None, slope=0.2):
     """-> dx like x, dgamma, dbeta (C,) fp32."""
-    B, N, C, groups, dt = sizes = _gn_sizes(x, gamma, beta, groups, act)
-    _chk(dy, x.dtype, "dy"); _chk(mean, F32, "mean"); _chk(rstd, F32, "rstd")
-    _chk_device("group_norm", dy, mean, rstd)
-    if dy.shape != x.shape or tuple(mean.shape) != (B, groups) or tuple(rstd.shape) != (B, groups):
-        raise RuntimeError("group_norm: dy, mean or rstd does not match x")
-    dx = torch.empty_like(x)
-    grads = torch.empty(2, C, dtype=F32, device=x.device)
-    ws = _gn_workspace(sizes, True, x.device)
+    B, N, C, groups, dt = _gn_sizes(x, gamma, beta, groups, act)
+    _chk(dy, x.dtype, "dy"); _chk(stats, F32, "stats")
+    if dy.shape != x.shape or stats.numel() != 2 * B * groups:
+        raise RuntimeError("group_norm: dy or the statistics do not match x")
+    stream = _launch_stream("group_norm", x, gamma, beta, dy, stats)
+    dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(beta)
+    ws = torch.empty(_gn_workspace_floats(B, N, C, groups, dt, 1), dtype=F32, device=x.device)
+    p = stats.data_ptr()
     rc = _timed("gn_bwd", 0, 3 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_bwd(
-        _ptr(x), _ptr(dy), _ptr(gamma), _ptr(beta), _ptr(mean), _ptr(rstd), _ptr(dx), _ptr(grads[0]), _ptr(grads[1]), _ptr(ws),
-        B, N, C, groups, dt, ACTS[act], float(slope), _stream()))
-    _lib.check(rc, "rgbd_group_norm_bwd")
-    return dx, grads[0], grads[1]
+        x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), p, p + 4 * B * groups, dx.data_ptr(), dgamma.data_ptr(),
+        dbeta.data_ptr(), ws.data_ptr(), B, N, C, groups, dt, ACTS[act], slope, stream))
+    if rc:
+        _lib.check(rc, "rgbd_group_norm_bwd")
+    return dx, dgamma, dbeta
 
 
 class _AttnDesc(ctypes.Structure):          # rgbd_attn_desc (include/rgbd_gan_hip.h)
@@ -1627,130 +1640,151 @@ class _AttnGrad(ctypes.Structure):          # rgbd_attn_grad
 HEAD_SIZES = (32, 64, 128)
 
 
-def attention_readable(t):
-    """Can the kernels read `t` (B, L, heads, D) as it lies: contiguous head vectors, 16-byte aligned."""
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t))
+class AttnOperands:
+    """Where q, k and v lie: sizes (B, H, Hkv, Lq, Lk, D), three addresses and nine strides (elements; an axis of one or no element has
+    stride 0, none that matters).  Made from three (B, tokens, heads, D) tensors or from one packed (B, N, (H + 2 Hkv) D)."""
+    __slots__ = ("sizes", "ptrs", "strides", "tensors")
+
+    @staticmethod
+    def _axis(t, n_axes=3):
+        return [s if n > 1 else 0 for s, n in zip(t.stride()[:n_axes], t.shape)]
+
+    @staticmethod
+    def readable(t, strides):
+        return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in strides)
+
+    @classmethod
+    def of(cls, q, k, v):
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            if not torch.is_tensor(t) or t.dim() != 4:
+                raise RuntimeError(f"attention: {name} must be (B, tokens, heads, head size)")
+            if t.dtype != BF16:
+                raise RuntimeError(f"attention: {name} must be bf16, got {t.dtype}")
+        B, Lq, H, D = q.shape
+        if D not in HEAD_SIZES:
+            raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
+        if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
+            raise RuntimeError(f"attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+        op = cls()
+        op.sizes, op.tensors, op.ptrs, op.strides = (B, H, k.shape[2], Lq, k.shape[1], D), (q, k, v), [], []
+        for t, name in ((q, "q"), (k, "k"), (v, "v")):
+            st = cls._axis(t)
+            if not cls.readable(t, st):
+                raise RuntimeError(f"attention: {name}: head vectors must be contiguous, strides multiples of 8, 16-byte aligned")
+            op.ptrs.append(t.data_ptr())
+            op.strides += st
+        return op
+
+    @classmethod
+    def packed(cls, qkv, heads, kv_heads):
+        if qkv.dtype != BF16:
+            raise RuntimeError(f"attention: qkv must be bf16, got {qkv.dtype}")
+        B, N, W = qkv.shape
+        D = W // (heads + 2 * kv_heads)
+        if D not in HEAD_SIZES:
+            raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
+        op = cls()
+        sb, sl = cls._axis(qkv, 2)
+        if not cls.readable(qkv, (sb, sl)):
+            raise RuntimeError("attention: qkv: a token's channels must be contiguous, strides multiples of 8, 16-byte aligned")
+        p = qkv.data_ptr()
+        op.sizes, op.tensors = (B, heads, kv_heads, N, N, D), (qkv,)
+        op.ptrs = [p, p + 2 * heads * D, p + 2 * (heads + kv_heads) * D] if p else [0, 0, 0]
+        op.strides = [sb, sl, D] * 3
+        return op
 
 
-def _strides(t):
-    """Strides of the first three axes; an axis of one (or no) element has none that matters."""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]
-
-
-def _attn_desc(q, k, v, table, buckets, lengths, scale, cap, q_start):
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if not torch.is_tensor(t) or t.dim() != 4:
-            raise RuntimeError(f"attention: {name} must be (B, tokens, heads, head size)")
-        if t.dtype != BF16:
-            raise RuntimeError(f"attention: {name} must be bf16, got {t.dtype}")
-    B, Lq, H, D = q.shape
-    if D not in HEAD_SIZES:
-        raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise RuntimeError(f"attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
-    Lk, Hkv = k.shape[1], k.shape[2]
+def _attn_desc(op, table, buckets, lengths, scale, cap, q_start, lse=0, fine=0):
+    B, H, Hkv, Lq, Lk, D = op.sizes
     if H < 1 or Hkv < 1 or H % Hkv:
         raise RuntimeError(f"attention: {Hkv} key / value heads do not divide {H} query heads")
     if not cap >= 0:
         raise RuntimeError(f"attention: cap must not be negative, got {cap}")
+    rows = cols = n_buckets = tab = bmap = lens = 0
     if (table is None) != (buckets is None):
         raise RuntimeError("attention: a bias table and its buckets come together")
-    rows = cols = n_buckets = 0
     if table is not None:
         rows, cols, n_buckets = buckets.rows, buckets.cols, buckets.n_buckets
-        if tuple(table.shape) != (H, n_buckets):
+        if table.shape != (H, n_buckets):
             raise RuntimeError(f"attention: table must be ({H}, {n_buckets}), got {tuple(table.shape)}")
         if rows > 1 and cols > 1024:
             raise RuntimeError(f"attention: a grid of more than one row has at most 1024 columns, got {cols}")
         if q_start < 0 or q_start + Lq > rows * cols or Lk > rows * cols:
             raise RuntimeError(f"attention: tokens outside the {rows} x {cols} grid (q_start {q_start}, {Lq} queries, {Lk} keys)")
+        _chk(table, F32, "table")
+        tab, bmap = table.data_ptr(), buckets.map.data_ptr()
     elif q_start:
         raise RuntimeError("attention: q_start places the queries on the bias's grid: it needs a table")
-    if lengths is not None and tuple(lengths.shape) != (B,):
-        raise RuntimeError(f"attention: lengths must be ({B},), got {tuple(lengths.shape)}")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        if not t.is_cuda:
-            raise RuntimeError(f"{name}: expected a GPU tensor (the HIP path has no CPU fallback)")
-        if not attention_readable(t):
-            raise RuntimeError(f"attention: {name}: head vectors must be contiguous, strides multiples of 8, 16-byte aligned")
-    _chk(table, F32, "table"); _chk(lengths, torch.int32, "lengths")
-    _chk_device("attention", q, k, v, table, lengths, buckets.map if buckets is not None else None)
-    d = _AttnDesc()
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.q_sb, d.q_sl, d.q_sh = _strides(q)
-    d.k_sb, d.k_sl, d.k_sh = _strides(k)
-    d.v_sb, d.v_sl, d.v_sh = _strides(v)
-    if table is not None:
-        d.table, d.map = table.data_ptr(), buckets.map.data_ptr()
     if lengths is not None:
-        d.lengths = lengths.data_ptr()
-    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D = B, H, Hkv, Lq, Lk, D
-    d.rows, d.cols, d.q_start, d.n_buckets = rows, cols, q_start, n_buckets
-    d.scale, d.cap = scale, cap
-    return d
+        if lengths.shape != (B,):
+            raise RuntimeError(f"attention: lengths must be ({B},), got {tuple(lengths.shape)}")
+        _chk(lengths, torch.int32, "lengths")
+        lens = lengths.data_ptr()
+    for t in op.tensors:
+        if not t.is_cuda:
+            raise RuntimeError("attention: expected a GPU tensor (the HIP path has no CPU fallback)")
+    stream = _launch_stream("attention", *op.tensors, table, lengths, buckets.map if buckets is not None else None)
+    return _AttnDesc(*op.ptrs, *op.strides, tab, bmap, lens, lse, B, H, Hkv, Lq, Lk, D, rows, cols, q_start, n_buckets, scale, cap,
+                     fine), stream
 
 
-def attention_fwd(q, k, v, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, keep=False, fine=False):
-    """q (B, Lq, H, D), k, v (B, Lk, Hkv, D) bf16 (attention_readable) -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward
-    pass needs: o_lo (what rounding o dropped, bf16) and lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient
-    needs of o (probabilities with 16 bits in the second product)."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    d = _attn_desc(q, k, v, table, buckets, lengths, scale, float(cap or 0.0), int(q_start))
-    o = torch.empty(d.B, d.Lq, d.H, d.D, dtype=BF16, device=q.device)
-    o_lo = lse = None
-    d.fine = int(fine)
-    if keep:
-        o_lo = torch.empty_like(o)
-        lse = torch.empty(d.B, d.H, d.Lq, dtype=F32, device=q.device)
-        d.lse = lse.data_ptr()
+_ATTN_WORKSPACE = {}                        # floats by sizes, grid and pass: what the library answers for them
+
+
+def _attn_workspace(op, buckets, q_start, kind, ask):
+    key = (*op.sizes, q_start, kind) if buckets is None else (*op.sizes, q_start, kind, buckets.rows, buckets.cols, buckets.n_buckets)
+    n = _ATTN_WORKSPACE.get(key)
+    if n is None:
+        n = ask()
+        if n < 0:
+            _lib.check(-1, "rgbd_attention workspace")
+        if len(_ATTN_WORKSPACE) > 1024:
+            _ATTN_WORKSPACE.clear()
+        _ATTN_WORKSPACE[key] = n
+    return n
+
+
+def attention_fwd(op, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, keep=False, fine=False):
+    """op: AttnOperands -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward pass needs: o_lo (what rounding o dropped, bf16) and
+    lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient needs of o (probabilities with 16 bits in the second product)."""
+    B, H, Hkv, Lq, Lk, D = op.sizes
+    t = op.tensors[0]
+    o = torch.empty((B, Lq, H, D), dtype=BF16, device=t.device)
+    o_lo = torch.empty_like(o) if keep else None
+    lse = torch.empty((B, H, Lq), dtype=F32, device=t.device) if keep else None
+    d, stream = _attn_desc(op, table, buckets, lengths, D ** -0.5 if scale is None else float(scale), cap, q_start,
+                           lse.data_ptr() if keep else 0, int(fine))
     lib = _lib.load()
-    n = lib.rgbd_attention_fwd_workspace(ctypes.byref(d))
-    if n < 0:
-        _lib.check(-1, "rgbd_attention_fwd_workspace")
-    ws = torch.empty(n, dtype=F32, device=q.device) if n else None
-    flops = 4 * d.B * d.H * d.Lq * d.Lk * d.D
-    rc = _timed("attn_fwd", flops, 4 * o.numel() + 4 * k.numel(), lambda: lib.rgbd_attention_fwd(
-        ctypes.byref(d), _ptr(o), _ptr(o_lo), _ptr(ws), _stream()))
-    _lib.check(rc, "rgbd_attention_fwd")
+    n = _attn_workspace(op, buckets, q_start, 0, lambda: lib.rgbd_attention_fwd_workspace(ctypes.byref(d)))
+    ws = torch.empty(n, dtype=F32, device=t.device) if n else None
+    rc = _timed("attn_fwd", 4 * B * H * Lq * Lk * D, 4 * B * D * (H * Lq + Hkv * Lk), lambda: lib.rgbd_attention_fwd(
+        ctypes.byref(d), o.data_ptr(), o_lo.data_ptr() if keep else 0, ws.data_ptr() if n else 0, stream))
+    if rc:
+        _lib.check(rc, "rgbd_attention_fwd")
     return o, o_lo, lse
 
 
-def attention_bwd(q, k, v, d_o, o, o_lo, lse, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, out=None,
-                  want_table=True):
-    """-> dq, dk, dv (views of `out` = three (B, L, heads, D) bf16 tensors where given), dtable (None unless wanted)."""
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
-    d = _attn_desc(q, k, v, table, buckets, lengths, scale, float(cap or 0.0), int(q_start))
+def attention_bwd(op, out, d_o, o, o_lo, lse, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, want_table=True):
+    """Writes dq, dk, dv where `out` (AttnOperands of the same sizes) says; -> dtable (None unless wanted)."""
+    B, H, Hkv, Lq, Lk, D = op.sizes
     for t, name in ((d_o, "d_o"), (o, "o"), (o_lo, "o_lo")):
         _chk(t, BF16, name)
-        if t.shape != q.shape:
-            raise RuntimeError(f"attention: {name} {tuple(t.shape)} does not match q {tuple(q.shape)}")
+        if t.shape != (B, Lq, H, D):
+            raise RuntimeError(f"attention: {name} {tuple(t.shape)} does not match q {(B, Lq, H, D)}")
     _chk(lse, F32, "lse")
-    if tuple(lse.shape) != (d.B, d.H, d.Lq):
-        raise RuntimeError(f"attention: lse must be {(d.B, d.H, d.Lq)}, got {tuple(lse.shape)}")
-    _chk_device("attention", d_o, o, o_lo, lse)
-    d.lse = lse.data_ptr()
-    if out is None:
-        out = tuple(torch.empty(t.shape, dtype=BF16, device=q.device) for t in (q, k, v))
-    for t, ref in zip(out, (q, k, v)):
-        if t.dtype != BF16 or t.shape != ref.shape or not attention_readable(t) or t.device != q.device:
-            raise RuntimeError("attention: a gradient buffer does not match its tensor")
+    if lse.shape != (B, H, Lq) or out.sizes != op.sizes:
+        raise RuntimeError("attention: lse or a gradient buffer does not match its tensor")
+    d, stream = _attn_desc(op, table, buckets, lengths, D ** -0.5 if scale is None else float(scale), cap, q_start, lse.data_ptr())
+    _launch_stream("attention", d_o, o, o_lo, lse, *out.tensors)
     want_table = bool(want_table and table is not None)
     dtable = torch.empty_like(table) if want_table else None
-    g = _AttnGrad()
-    g.d_o, g.o, g.o_lo = d_o.data_ptr(), o.data_ptr(), o_lo.data_ptr()
-    g.dq, g.dk, g.dv = (t.data_ptr() for t in out)
-    g.dq_sb, g.dq_sl, g.dq_sh = _strides(out[0])
-    g.dk_sb, g.dk_sl, g.dk_sh = _strides(out[1])
-    g.dv_sb, g.dv_sl, g.dv_sh = _strides(out[2])
-    if want_table:
-        g.dtable, g.order, g.start = dtable.data_ptr(), buckets.order.data_ptr(), buckets.start.data_ptr()
+    g = _AttnGrad(d_o.data_ptr(), o.data_ptr(), o_lo.data_ptr(), *out.ptrs, *out.strides, *(
+        (dtable.data_ptr(), buckets.order.data_ptr(), buckets.start.data_ptr()) if want_table else (0, 0, 0)))
     lib = _lib.load()
-    n = lib.rgbd_attention_bwd_workspace(ctypes.byref(d), int(want_table))
-    if n < 0:
-        _lib.check(-1, "rgbd_attention_bwd_workspace")
-    ws = torch.empty(n, dtype=F32, device=q.device)
-    flops = 10 * d.B * d.H * d.Lq * d.Lk * d.D
-    rc = _timed("attn_bwd", flops, 8 * q.numel() + 8 * k.numel(), lambda: lib.rgbd_attention_bwd(
-        ctypes.byref(d), ctypes.byref(g), _ptr(ws), _stream()))
-    _lib.check(rc, "rgbd_attention_bwd")
-    return (*out, dtable)
+    n = _attn_workspace(op, buckets, q_start, 1 + want_table, lambda: lib.rgbd_attention_bwd_workspace(ctypes.byref(d), int(want_table)))
+    ws = torch.empty(n, dtype=F32, device=d_o.device)
+    rc = _timed("attn_bwd", 10 * B * H * Lq * Lk * D, 8 * B * D * (H * Lq + Hkv * Lk), lambda: lib.rgbd_attention_bwd(
+        ctypes.byref(d), ctypes.byref(g), ws.data_ptr(), stream))
+    if rc:
+        _lib.check(rc, "rgbd_attention_bwd")
+    return dtable
