@@ -67,6 +67,15 @@ struct GnArgs {
     float eps, slope;
 };
 
+// Groups of V neighbouring channels from c on: one division, then counted.
+template <int V> __device__ __forceinline__ void groups_of(int (&g)[V], int c, int cpg) {
+    int q = c / cpg, r = c - q * cpg;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        g[i] = q;
+        if (++r == cpg) { r = 0; ++q; }
+    }
+}
 __device__ __forceinline__ float fast_sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
 }
@@ -81,8 +90,39 @@ template <int ACT> __device__ __forceinline__ float act_grad(float z, float slop
     return 1.f;
 }
 
-// Sums of v[0..V) over the workgroup's pixel lanes: red is (pl, cw) fp32, the channel sums end in red[0 .. cw).
+// Sums of v[0..V) over the workgroup's pixel lanes: the channel sums end in red[0 .. cw).  Where the vectors of a pixel divide a wave, a
+// wave adds up its own pixels with shuffles and a thread a channel adds the waves (two barriers; red: a row a wave); else by halves
+// (red: a row a pixel lane).
 template <int V> __device__ __forceinline__ void sum_over_pixels(float* red, const float* v, int p, int j, int pl, int cw, bool live) {
+    const int nc = cw / V;
+    if ((nc & (nc - 1)) == 0 && nc <= 64) {
+        float w[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) w[i] = live ? v[i] : 0.f;
+        for (int off = 32; off >= nc; off >>= 1)
+#pragma unroll
+            for (int i = 0; i < V; ++i) w[i] += __shfl_xor(w[i], off, 64);
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+        if (lane < nc)
+#pragma unroll
+            for (int i = 0; i < V; ++i) red[wave * cw + lane * V + i] = w[i];
+        __syncthreads();
+        float s = 0.f;
+        const int c = threadIdx.x;
+        if (c < cw)
+            for (int k = 0; k < waves; ++k) s += red[k * cw + c];
+        float t[7];                                        // (cw <= 64 V = 512: one channel a thread of 64 .. 1024, more where threads are fewer)
+        for (int e = 1; c + e * (int)blockDim.x < cw; ++e) {
+            float q = 0.f;
+            for (int k = 0; k < waves; ++k) q += red[k * cw + c + e * blockDim.x];
+            t[e - 1] = q;
+        }
+        __syncthreads();
+        if (c < cw) red[c] = s;
+        for (int e = 1; c + e * (int)blockDim.x < cw; ++e) red[c + e * blockDim.x] = t[e - 1];
+        __syncthreads();
+        return;
+    }
     if (live)
 #pragma unroll
         for (int i = 0; i < V; ++i) red[p * cw + j * V + i] = v[i];
@@ -97,14 +137,23 @@ template <int V> __device__ __forceinline__ void sum_over_pixels(float* red, con
     }
 }
 
-// Sum of ch[g * cpg .. + cpg) (LDS) for every group of the workgroup, a wave per group in turn -> out[g] (LDS).
+// Sum of ch[g * cpg .. + cpg) (LDS) for every group of the workgroup -> out[g] (LDS): a thread a group while that is a few adds, else a
+// wave a group in turn.
 __device__ __forceinline__ void sum_over_group(const float* ch, float* out, int groups, int cpg) {
     const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
-    for (int g = threadIdx.x >> 6; g < groups; g += nw) {
-        float s = 0.f;
-        for (int i = lane; i < cpg; i += 64) s += ch[g * cpg + i];
-        s = wave_sum(s);
-        if (lane == 0) out[g] = s;
+    if (cpg <= 32) {
+        for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+            float s = 0.f;
+            for (int i = 0; i < cpg; ++i) s += ch[g * cpg + i];
+            out[g] = s;
+        }
+    } else {
+        for (int g = threadIdx.x >> 6; g < groups; g += nw) {
+            float s = 0.f;
+            for (int i = lane; i < cpg; i += 64) s += ch[g * cpg + i];
+            s = wave_sum(s);
+            if (lane == 0) out[g] = s;
+        }
     }
     __syncthreads();
 }
@@ -139,9 +188,11 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(GnArgs a) {
     sum_over_group(red, gm, groups, a.cpg);
     const float inv = 1.f / ((float)a.N * (float)a.cpg);
     float mean[V], gamma[V], beta[V];
+    int gi[V];
+    groups_of<V>(gi, live ? j * V : 0, a.cpg);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        mean[i] = live ? gm[(j * V + i) / a.cpg] * inv : 0.f;
+        mean[i] = live ? gm[gi[i]] * inv : 0.f;
         gamma[i] = live ? a.gamma[c0 + j * V + i] : 0.f;
         beta[i] = live ? a.beta[c0 + j * V + i] : 0.f;
         acc[i] = 0.f;
@@ -161,7 +212,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(GnArgs a) {
     if (!live) return;
     float scale[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) scale[i] = 1.f / sqrtf(gr[(j * V + i) / a.cpg] * inv + a.eps);
+    for (int i = 0; i < V; ++i) scale[i] = 1.f / sqrtf(gr[gi[i]] * inv + a.eps);
     T* y = reinterpret_cast<T*>(a.out) + (int64_t)b * a.N * a.C + c0 + j * V;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -196,11 +247,14 @@ __global__ __launch_bounds__(1024) void gn_bwd_resident(GnArgs a) {
         else { xs[e].zero(); ds[e].zero(); }
     }
     float mean[V], rstd[V], gamma[V], beta[V], sa[V], sb[V];
+    int gi[V];
+    groups_of<V>(gi, live ? j * V : 0, a.cpg);
+    const int64_t g0 = (int64_t)b * a.G + c0 / a.cpg;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = c0 + (live ? j * V + i : 0);
-        mean[i] = a.mean[(int64_t)b * a.G + c / a.cpg];
-        rstd[i] = a.rstd[(int64_t)b * a.G + c / a.cpg];
+        mean[i] = a.mean[g0 + gi[i]];
+        rstd[i] = a.rstd[g0 + gi[i]];
         gamma[i] = a.gamma[c];
         beta[i] = a.beta[c];
         sa[i] = sb[i] = 0.f;
@@ -233,7 +287,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_resident(GnArgs a) {
     const float inv = 1.f / ((float)a.N * (float)a.cpg);
     float m1[V], m2[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) { m1[i] = s1[(j * V + i) / a.cpg] * inv; m2[i] = s2[(j * V + i) / a.cpg] * inv; }
+    for (int i = 0; i < V; ++i) { m1[i] = s1[gi[i]] * inv; m2[i] = s2[gi[i]] * inv; }
     T* dx = reinterpret_cast<T*>(a.out) + base;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -355,9 +409,11 @@ __global__ __launch_bounds__(1024) void gn_slab_apply(GnArgs a) {
     const int p = threadIdx.x / a.nc, j = threadIdx.x - p * a.nc;
     if (p >= a.pl) return;
     float sc[V], sh[V];
+    int gi[V];
+    groups_of<V>(gi, j * V, a.cpg);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = j * V + i, g = c / a.cpg;
+        const int c = j * V + i, g = gi[i];
         sc[i] = gr[g] * a.gamma[c];
         sh[i] = gm[g];
     }
@@ -397,11 +453,13 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_sums(GnArgs a) {
     const T* x = reinterpret_cast<const T*>(a.x) + base;
     const T* dy = reinterpret_cast<const T*>(a.dy) + base;
     float mean[V], rstd[V], gamma[V], beta[V], sa[V], sb[V];
+    int gi[V];
+    groups_of<V>(gi, live ? j * V : 0, a.cpg);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const int c = live ? j * V + i : 0;
-        mean[i] = a.mean[(int64_t)b * a.G + c / a.cpg];
-        rstd[i] = a.rstd[(int64_t)b * a.G + c / a.cpg];
+        mean[i] = a.mean[(int64_t)b * a.G + gi[i]];
+        rstd[i] = a.rstd[(int64_t)b * a.G + gi[i]];
         gamma[i] = a.gamma[c];
         beta[i] = a.beta[c];
         sa[i] = sb[i] = 0.f;
@@ -445,37 +503,51 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_sums(GnArgs a) {
     }
 }
 
-// dgamma / dbeta of 32 channels from `rows` partial rows of (C, 2): 8 row lanes a channel half, joined in a fixed order.
+// dgamma / dbeta of 8 channels from `rows` partial rows of (C, 2): a row lane for every 16 threads, eight rows at a time, joined in a fixed
+// order.
+constexpr int PG = 8;
 __device__ void param_grads(const float* part, int64_t rows, int C, int c0, float* dgamma, float* dbeta, float* red) {
-    const int col = threadIdx.x & 63;                      // (channel, which) of 32 channels
-    const int lanes = blockDim.x >> 6, r0 = threadIdx.x >> 6;
+    const int col = threadIdx.x & 15;                      // (channel, which) of 8 channels
+    const int lanes = blockDim.x >> 4, r0 = threadIdx.x >> 4;
     const bool in = c0 * 2 + col < 2 * C;
     float s = 0.f;
     if (in)
-        for (int64_t r = r0; r < rows; r += lanes) s += part[r * 2 * C + c0 * 2 + col];
+        for (int64_t r = r0; r < rows; r += 8 * lanes) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int64_t q = r + k * lanes;
+                v[k] = part[(q < rows ? q : rows - 1) * 2 * C + c0 * 2 + col];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += r + k * lanes < rows ? v[k] : 0.f;
+        }
     red[threadIdx.x] = s;
     __syncthreads();
     if (r0 == 0 && in) {
-        for (int k = 1; k < lanes; ++k) s += red[k * 64 + col];
+        for (int k = 1; k < lanes; ++k) s += red[k * 16 + col];
         if (col & 1) dgamma[c0 + (col >> 1)] = s;
         else dbeta[c0 + (col >> 1)] = s;
     }
 }
 
-__global__ __launch_bounds__(1024) void gn_param_grads(const float* part, int64_t rows, int C, float* dgamma, float* dbeta) {
-    __shared__ float red[1024];
-    param_grads(part, rows, C, blockIdx.x * 32, dgamma, dbeta, red);
+__global__ __launch_bounds__(256) void gn_param_grads(const float* part, int64_t rows, int C, float* dgamma, float* dbeta) {
+    __shared__ float red[256];
+    param_grads(part, rows, C, blockIdx.x * PG, dgamma, dbeta, red);
 }
 
-// grid.x = apply_wgs workgroups that write dx (each sample), then, of sample 0, ceil(C / 32) that sum the parameters' gradients.
+// grid.x = ceil(C / 8) workgroups that sum the parameters' gradients (of sample 0: a long chain of adds, so they start first), then
+// apply_wgs that write dx.
 template <typename T, int V, int ACT>
 __global__ __launch_bounds__(1024) void gn_slab_bwd_apply(GnArgs a) {
     extern __shared__ float lds[];                        // s1 (G) | s2 (G), or red (blockDim)
     const int b = blockIdx.y;
-    if ((int)blockIdx.x >= a.apply_wgs) {
-        if (b == 0) param_grads(a.part, (int64_t)a.B * a.slabs, a.C, (blockIdx.x - a.apply_wgs) * 32, a.dgamma, a.dbeta, lds);
+    const int first = (a.C + PG - 1) / PG;
+    if ((int)blockIdx.x < first) {
+        if (b == 0) param_grads(a.part, (int64_t)a.B * a.slabs, a.C, blockIdx.x * PG, a.dgamma, a.dbeta, lds);
         return;
     }
+    const int wg = blockIdx.x - first;
     float* s1 = lds;
     float* s2 = lds + a.G;
     const int lane = threadIdx.x & 63, nw = blockDim.x >> 6;
@@ -495,9 +567,11 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_apply(GnArgs a) {
     const int p = threadIdx.x / a.nc, j = threadIdx.x - p * a.nc;
     if (p >= a.pl) return;
     float mean[V], rstd[V], gamma[V], beta[V], m1[V], m2[V];
+    int gi[V];
+    groups_of<V>(gi, j * V, a.cpg);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int c = j * V + i, g = c / a.cpg;
+        const int c = j * V + i, g = gi[i];
         mean[i] = a.mean[(int64_t)b * a.G + g];
         rstd[i] = a.rstd[(int64_t)b * a.G + g];
         gamma[i] = a.gamma[c];
@@ -511,7 +585,7 @@ __global__ __launch_bounds__(1024) void gn_slab_bwd_apply(GnArgs a) {
     T* dx = reinterpret_cast<T*>(a.out) + base;
     constexpr int U = 4;
     const int step = a.pl * a.apply_wgs;
-    for (int n = blockIdx.x * a.pl + p; n < a.N; n += U * step) {
+    for (int n = wg * a.pl + p; n < a.N; n += U * step) {
         Vec<T, V> xs[U], ds[U];
 #pragma unroll
         for (int u = 0; u < U; ++u)
@@ -617,12 +691,12 @@ template <typename T, int V, int ACT> void launch_bwd(const GnPlan& p, GnArgs& a
         const size_t lds = (size_t)(p.pl * p.cw + 2 * (p.cw / a.cpg)) * 4;
         if (p.e <= 2) hipLaunchKernelGGL((gn_bwd_resident<T, V, 2, ACT>), grid, dim3(p.threads), lds, s, a);
         else hipLaunchKernelGGL((gn_bwd_resident<T, V, 4, ACT>), grid, dim3(p.threads), lds, s, a);
-        hipLaunchKernelGGL(gn_param_grads, dim3(ceil_div(a.C, 32)), dim3(512), 0, s, a.part, (int64_t)a.B, a.C, a.dgamma, a.dbeta);
+        hipLaunchKernelGGL(gn_param_grads, dim3(ceil_div(a.C, PG)), dim3(256), 0, s, a.part, (int64_t)a.B, a.C, a.dgamma, a.dbeta);
         return;
     }
     hipLaunchKernelGGL((gn_slab_bwd_sums<T, V, ACT>), dim3(a.slabs, a.B), dim3(p.threads), (size_t)p.pl * a.C * 4, s, a);
     const size_t lds = (size_t)(2 * a.G > p.threads ? 2 * a.G : p.threads) * 4;
-    hipLaunchKernelGGL((gn_slab_bwd_apply<T, V, ACT>), dim3(a.apply_wgs + ceil_div(a.C, 32), a.B), dim3(p.threads), lds, s, a);
+    hipLaunchKernelGGL((gn_slab_bwd_apply<T, V, ACT>), dim3(a.apply_wgs + ceil_div(a.C, PG), a.B), dim3(p.threads), lds, s, a);
 }
 
 template <typename T, int V> void by_act(bool bwd, int act, const GnPlan& p, GnArgs& a, hipStream_t s) {
