@@ -154,6 +154,14 @@ template <int N> __device__ __forceinline__ void arrived(bf16x8 (&f)[N]) {
     }
 }
 
+// What rounding a value to bf16 drops, in 16 bits and all of it: fp32's low half.  hi is the nearest, so the value's bits are hi * 2^16 +
+// the low half read as a signed number; a tie goes to the even hi, and one that went down is stored a unit lower (2^-24 of the value).
+__device__ __forceinline__ unsigned low_half(float v) {
+    const unsigned b = __float_as_uint(v);
+    return (b & 0x1ffffu) == 0x8000u ? 0x7fffu : b & 0xffffu;
+}
+__device__ __forceinline__ float whole(unsigned hi, unsigned lo) { return __uint_as_float((hi << 16) + (unsigned)(int)(short)lo); }
+
 // tanh of 16 values.  Below 0.5 an odd polynomial (least squares on Chebyshev nodes, relative error 1.1e-7: there the quotient
 // form would lose digits by cancellation, and capped scores mostly lie there); beyond it 1 - 2 / (e^2x + 1).
 __device__ __forceinline__ float tanh_small(float x) {
@@ -483,9 +491,8 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
             for (int i = 0; i < 4; ++i) f[i] = o[d][4 * g + i] * il;
             const u32x2 w = {pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3])};
             *reinterpret_cast<u32x2*>(a.out + ob + 32 * d + 8 * g) = w;
-            if (a.out_lo) {                                          // what the rounding dropped: delta needs more than bf16
-                const u32x2 r = {pack_bf16x2(f[0] - bf16_lo(w[0]), f[1] - bf16_hi(w[0])),
-                                 pack_bf16x2(f[2] - bf16_lo(w[1]), f[3] - bf16_hi(w[1]))};
+            if (a.out_lo) {                                          // delta needs o in fp32
+                const u32x2 r = {low_half(f[0]) | low_half(f[1]) << 16, low_half(f[2]) | low_half(f[3]) << 16};
                 *reinterpret_cast<u32x2*>(a.out_lo + ob + 32 * d + 8 * g) = r;
             }
         }
@@ -694,7 +701,7 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
     const float l = row_l, y = l > 0.f ? s / l : (l == 0.f ? 0.f : l);
     const int64_t at = (int64_t)blockIdx.x * D + d;
     a.out[at] = f32_to_bf16_bits(y);
-    if (a.out_lo) a.out_lo[at] = f32_to_bf16_bits(y - bf16_bits_to_f32(f32_to_bf16_bits(y)));
+    if (a.out_lo) a.out_lo[at] = (unsigned short)low_half(y);
     if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + qi] = l == 0.f ? 0.f : row_m + __builtin_amdgcn_logf(l);
 }
 
@@ -746,10 +753,12 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
         for (int ks = 0; ks < KS; ++ks) {
             qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
             gf[ks] = *reinterpret_cast<const bf16x8*>(a.d_o + ob + 16 * ks);
-            const bf16x8 ov = *reinterpret_cast<const bf16x8*>(a.o + ob + 16 * ks);
-            const bf16x8 lv = *reinterpret_cast<const bf16x8*>(a.o_lo + ob + 16 * ks);
+            const u32x4 ov = *reinterpret_cast<const u32x4*>(a.o + ob + 16 * ks), lv = *reinterpret_cast<const u32x4*>(a.o_lo + ob + 16 * ks);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) delta += (float)gf[ks][i] * ((float)ov[i] + (float)lv[i]);
+            for (int i = 0; i < 4; ++i) {
+                delta += (float)gf[ks][2 * i] * whole(ov[i] & 0xffffu, lv[i]);
+                delta += (float)gf[ks][2 * i + 1] * whole(ov[i] >> 16, lv[i] >> 16);
+            }
         }
     }
     delta = other_half_sum(delta);

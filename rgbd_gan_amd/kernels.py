@@ -1745,7 +1745,7 @@ def _attn_workspace(op, buckets, q_start, kind, ask):
 
 
 def attention_fwd(op, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, keep=False, fine=False):
-    """op: AttnOperands -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward pass needs: o_lo (what rounding o dropped, bf16) and
+    """op: AttnOperands -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward pass needs: o_lo (the low 16 bits of o's fp32 values, typed bf16) and
     lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient needs of o (probabilities with 16 bits in the second product)."""
     B, H, Hkv, Lq, Lk, D = op.sizes
     t = op.tensors[0]
