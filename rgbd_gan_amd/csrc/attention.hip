@@ -23,10 +23,12 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 // rows of a streamed tile (keys forward and in dq, queries in dk / dv): two buffers of two operands are 32 KB of LDS either way
 constexpr int kt_of(int D) { return D == 128 ? 32 : 64; }
+// ... of dq, which has the table's gradient in LDS too: 16 or 32 KB, three workgroups a compute unit at head sizes up to 64
+constexpr int kt_dq(int D) { return D == 128 ? 32 : 64; }
 constexpr int BLK = 128;                  // rows a workgroup owns: 4 waves x 32
 constexpr int WIN_PAD = 4;
 // LDS bytes for the window: next to the tiles of two workgroups of head size 64 (32 KB each, 69 KB with ds blocks) in 160 KB
-constexpr int WIN_FWD = 20480, WIN_DQ = 11264;
+constexpr int WIN_FWD = 20480, WIN_DQ = 10240;
 constexpr float NO_ROW = 0x1p100f;          // log2-sum-exp of a row that is not there: p = exp2(x - 2^100) = 0 for every finite x
 constexpr float NEG_INF = -__builtin_inff();
 
@@ -88,8 +90,8 @@ template <int D> struct Frags {
 // row; the permutation of the chunks is in the source addresses).  Rows at or beyond `valid` repeat the last valid one: whatever
 // memory holds there, a NaN included, is never read.  M0 carries the LDS address; nothing the compiler emits for gfx950 reads it.
 // The caller waits with dma_wait() before the barrier that publishes the tile.
-template <int D> struct Dma {
-    static constexpr int KT = kt_of(D), CH = D / 8, NP = KT * CH / 256;
+template <int D, int KT> struct Dma {
+    static constexpr int CH = D / 8, NP = KT * CH / 256;
     unsigned off[NP];                     // bytes from the tile's first row
     int64_t step;                         // bytes of KT rows
     const char* base;
@@ -362,7 +364,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
     float m = 0.f, l = 0.f;
     bool moved = false;                                              // (of the wave) some m is not 0
 
-    Dma<D> sk, sv;
+    Dma<D, KT> sk, sv;
     Places<BIAS> pl;
     int seg_t = 0;                                                   // the first tile of the segment in the window
     if (BIAS) pl.init(a, 0);
@@ -719,13 +721,14 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
 // LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
 enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
 constexpr int BS = 72;                    // floats from row to row of a block: rows 4 apart (a wave's halves) are 32 banks apart
-constexpr int BLOCK_FLOATS = 32 + 32 * BS;
-constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * BLOCK_FLOATS * 4 : dt == DT_DIAGONALS ? kt_of(D) * BLK * 4 : 0; }
+constexpr int block_rows(int D) { return D == 128 ? 16 : 32; }       // (16: a block goes through in two halves, for two workgroups' LDS)
+constexpr int block_floats(int D) { return 32 + block_rows(D) * BS; }
+constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * block_floats(D) * 4 : dt == DT_DIAGONALS ? kt_dq(D) * BLK * 4 : 0; }
 
 template <int D, int BIAS, bool CAP, int DT>
 __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int KT = kt_of(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    constexpr int BR = block_rows(D), KT = kt_dq(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
     float* dsl = reinterpret_cast<float*>(smem + 4 * TB);
     char* win = smem + 4 * TB + dt_lds(DT, D);
     int* at = reinterpret_cast<int*>(win + a.win_bytes);
@@ -737,9 +740,9 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
     const int row = qb * BLK + wave * 32 + (lane & 31);
     const bool live = row < a.Lq;
     const Frags<D> fr(lane);
-    float* blk = dsl + wave_id() * BLOCK_FLOATS + 32;                // BLOCKS: row 0, zeros in front of it
+    float* blk = dsl + wave_id() * block_floats(D) + 32;                // BLOCKS: row 0, zeros in front of it
     if (DT == DT_BLOCKS) {
-        for (int i = lane; i < BLOCK_FLOATS; i += 64) blk[i - 32] = 0.f;
+        for (int i = lane; i < block_floats(D); i += 64) blk[i - 32] = 0.f;
         wave_fence();
     }
 
@@ -782,8 +785,10 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
     float* part = DT == DT_DIAGONALS ? a.part + (int64_t)id * 2 * a.span
                                      : DT == DT_BLOCKS ? a.part + ((int64_t)id * 4 + wave) * n_kg * 64 : nullptr;
     const int d_min = tq0 - (nt * KT - 1);
+    float hold[KT / 32];                                             // BLOCKS: a tile's sums, stored a tile later: the wait for the next tile's
+                                                                     // loads would wait for a store that has just gone out
 
-    Dma<D> sk, sv;
+    Dma<D, KT> sk, sv;
     Places<BIAS> pl;
     int seg_t = 0;
     if (BIAS) pl.init(a, 0);
@@ -809,6 +814,9 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             Places<BIAS>::table(at, a, t * KT, n, a.Lk - 1);
         }
         __syncthreads();
+        if (DT == DT_BLOCKS && t > 0)
+#pragma unroll
+            for (int u = 0; u < KT / 32; ++u) part[(KT / 32 * (t - 1) + u) * 64 + lane] = hold[u];
         if (t + 1 < nt) {
             sk.next(a.k_sl, (P ^ 1) * TB);
             sv.next(a.v_sl, (P ^ 1) * TB);
@@ -825,8 +833,6 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             if (BIAS) pl.next();
             PHASE();
             f32x16 dp = f.times(gf, splat(0.f));
-            ColOps<D> kt;
-            kt.load(fr, kc, 32 * u);
             PHASE();
             to_logits<BIAS, CAP>(s, th, a, bias);
             if (t * KT + KT > len) {
@@ -840,22 +846,42 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             for (int i = 0; i < 16; ++i) {
                 const float ds = __builtin_amdgcn_exp2f(s[i] - lse) * (dp[i] - delta);
                 if (DT == DT_DIAGONALS) dsl[(32 * u + 8 * (i >> 2) + 4 * half + (i & 3)) * BLK + wave * 32 + (lane & 31)] = ds;
-                if (DT == DT_BLOCKS) blk[(8 * (i >> 2) + 4 * half + (i & 3)) * BS + (lane & 31)] = ds;
+                dp[i] = ds;
                 s[i] = CAP ? ds * (1.f - th[i] * th[i]) : ds;
             }
+            ColOps<D> kt;
+            kt.load(fr, kc, 32 * u);
+            // the table's sums: the block's values go out and its diagonals come in while the products run
+            float diag[32];
+            auto put = [&](int e) {
+#pragma unroll
+                for (int i = 0; i < BR / 2; ++i) blk[(8 * (i >> 2) + 4 * half + (i & 3)) * BS + (lane & 31)] = dp[BR / 2 * e + i];
+                wave_fence();
+            };
+            auto get = [&](int e) {                                  // lane: query - key = lane - 32
+#pragma unroll
+                for (int i = 0; i < BR; ++i) diag[i] = blk[i * (BS + 1) + BR * e + lane - 32];
+                wave_fence();
+            };
+            auto total = [&] {
+                float t4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < BR; ++i) t4[i & 3] += diag[i];
+                return (t4[0] + t4[1]) + (t4[2] + t4[3]);
+            };
+            if (DT == DT_BLOCKS) { put(0); get(0); }
+            PHASE();
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const bf16x8 pf = pack8(s, 8 * g);
 #pragma unroll
                 for (int d = 0; d < DB; ++d) acc[d] = mfma(kt.f[g][d], pf, acc[d]);
             }
-            if (DT == DT_BLOCKS) {                                   // lane: query - key = lane - 32
-                wave_fence();
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) sum += blk[i * (BS + 1) + lane - 32];
-                part[(KT / 32 * t + u) * 64 + lane] = sum;
-                wave_fence();
+            if (DT == DT_BLOCKS) {
+                PHASE();
+                float sum = total();
+                if (BR == 16) { put(1); get(1); sum += total(); }
+                hold[u] = sum;
             }
         }
         dma_wait();
@@ -895,6 +921,9 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
         tile(t, std::integral_constant<int, 0>{});
         if (t + 1 < nt) tile(t + 1, std::integral_constant<int, 1>{});
     }
+    if (DT == DT_BLOCKS && nt > 0)
+#pragma unroll
+        for (int u = 0; u < KT / 32; ++u) part[(KT / 32 * (nt - 1) + u) * 64 + lane] = hold[u];
     if (!live) return;
     unsigned short* qo = a.dq + b * a.dq_sb + (int64_t)row * a.dq_sl + h * a.dq_sh + 4 * half;
 #pragma unroll
@@ -1054,7 +1083,7 @@ __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_
         const int nqt = (a.Lq + KT - 1) / KT;
         const float neg_inv_f = -1.f / (a.scale * LOG2E);
 
-        Dma<D> sq, sg;
+        Dma<D, KT> sq, sg;
         float next_l = 0.f, next_d = 0.f;
         auto load = [&](int h, int t, int buf, bool first) {          // tile t of head h into buffer buf
             if (t == 0 || first) {
@@ -1360,7 +1389,7 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     const int ks = kv_splits(d);
     z.kv = ks > 1 ? (int64_t)ks * d->B * d->Hkv * d->Lk * 2 * d->D : 0;
     if (!dt || d->Lq == 0 || d->Lk == 0) return z;
-    const int KT = kt_of(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
+    const int KT = kt_dq(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
         z.mode = DT_BLOCKS;
         z.part = (int64_t)d->B * d->H * n_qb * 4 * n_kt * (KT / 32) * 64;
@@ -1466,6 +1495,8 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
 
     if (d->Lq > 0) {
         const int bias = bias_mode(d, 0);
+        a.kt = kt_dq(d->D);
+        a.n_kt = ceil_div(d->Lk, a.kt);
         const Window w = window_of(bias, d->Lq, d->Lk, a.rows, a.cols, a.kt, z.mode ? WIN_DQ : WIN_FWD);
         RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
         a.seg_tiles = w.tiles;
@@ -1489,6 +1520,7 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
     if (z.mode) RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
     if (d->Lk > 0) {
         const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
+        a.kt = kt_of(d->D);
         const Window w = window_of(bias, d->Lk, d->Lq, a.rows, a.cols, a.kt, WIN_FWD);
         RGBD_REQUIRE(bias == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
         a.seg_tiles = w.tiles;
