@@ -27,7 +27,7 @@ constexpr int kt_of(int D) { return D == 128 ? 32 : 64; }
 constexpr int kt_dq(int D) { return D == 128 ? 32 : 64; }
 constexpr int BLK = 128;                  // rows a workgroup owns: 4 waves x 32
 constexpr int WIN_PAD = 4;
-// LDS bytes for the window: next to the tiles of two workgroups of head size 64 (32 KB each, 69 KB with ds blocks) in 160 KB
+// LDS bytes for the window: with the tiles (32 KB) three workgroups a compute unit forward, two of dq with its blocks (69 KB)
 constexpr int WIN_FWD = 20480, WIN_DQ = 10240;
 constexpr float NO_ROW = 0x1p100f;          // log2-sum-exp of a row that is not there: p = exp2(x - 2^100) = 0 for every finite x
 constexpr float NEG_INF = -__builtin_inff();
@@ -198,6 +198,10 @@ __device__ __forceinline__ int xcd_run(int id, int total) {
     return x * q + min(x, r) + (id >> 3);
 }
 
+// A bias in the exponent of 2.  One at or below -1e30 (a mask written as the type's lowest number) is -inf: a row that has nothing else
+// would otherwise carry a log-sum-exp in which the sum is below the last digit, and its gradients would be wrong.
+__device__ __forceinline__ float in_log2(float bias) { return bias <= -1e30f ? NEG_INF : bias * LOG2E; }
+
 // ---- the bias of a run of tiles (a segment), in LDS.  The workgroup's own rows are tokens at places own_first .. own_last, the
 //      streamed ones begin at other_first and span `span` places.  Entry j is the offset whose place grows with the streamed row, so a
 //      lane reads upwards; SIGN +1: the streamed rows are queries.  Values are kept times log2(e): the softmax runs on exp2.
@@ -210,7 +214,7 @@ __device__ __forceinline__ void stage_window(float* win, const AttnArgs& a, int 
     for (int j = threadIdx.x; j < n; j += 256) {
         const int e = base + SIGN * j;                                // beyond the map: a streamed row that is no token
         const int u = min(max(a.map[min(max(e, 0), size - 1)], 0), a.n_buckets - 1);
-        win[j] = e >= 0 && e < size ? row[u] * LOG2E : 0.f;
+        win[j] = e >= 0 && e < size ? in_log2(row[u]) : 0.f;
     }
 }
 
@@ -253,8 +257,7 @@ template <int BIAS> struct Places {
 // 16 biases of a lane: rows 8 (i / 4) + 4 half + i % 4 of a block of 32; `at`: the block's rows in the table of BIAS 1.
 template <int BIAS>
 __device__ __forceinline__ f32x16 read_bias(const char* win, const Places<BIAS>& pl, const int* at, int half, int lane_off) {
-    f32x16 o;
-    if (BIAS == 0) return o;
+    f32x16 o = {};
     if (BIAS == 2) {
         const char* w0 = win + (lane_off + pl.blk);
 #pragma unroll
@@ -263,7 +266,7 @@ __device__ __forceinline__ f32x16 read_bias(const char* win, const Places<BIAS>&
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[4 * g + i] = w[i];
         }
-    } else {
+    } else if (BIAS == 1) {
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -561,7 +564,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     };
     auto buckets = [&] {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) bias[i] = trow[min(max(u[i], 0), a.n_buckets - 1)] * LOG2E;
+        for (int i = 0; i < 16; ++i) bias[i] = in_log2(trow[min(max(u[i], 0), a.n_buckets - 1)]);
     };
 
     bf16x8 qf[KS];
@@ -821,19 +824,15 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             sk.next(a.k_sl, (P ^ 1) * TB);
             sv.next(a.v_sl, (P ^ 1) * TB);
         }
-        PHASE();
 #pragma unroll
         for (int u = 0; u < KT / 32; ++u) {
             RowOps<D> f;
             f.load(fr, kc, 32 * u);
-            PHASE();
             f32x16 s = f.times(qf, splat(0.f)), th;
             f.load(fr, vc, 32 * u);
             const f32x16 bias = read_bias<BIAS>(win, pl, at + (t - seg_t) * KT + 32 * u, half, lane_off);
             if (BIAS) pl.next();
-            PHASE();
             f32x16 dp = f.times(gf, splat(0.f));
-            PHASE();
             to_logits<BIAS, CAP>(s, th, a, bias);
             if (t * KT + KT > len) {
                 int k0 = t * KT + 32 * u + 4 * half;
@@ -870,7 +869,6 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
                 return (t4[0] + t4[1]) + (t4[2] + t4[3]);
             };
             if (DT == DT_BLOCKS) { put(0); get(0); }
-            PHASE();
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const bf16x8 pf = pack8(s, 8 * g);
@@ -878,7 +876,6 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
                 for (int d = 0; d < DB; ++d) acc[d] = mfma(kt.f[g][d], pf, acc[d]);
             }
             if (DT == DT_BLOCKS) {
-                PHASE();
                 float sum = total();
                 if (BR == 16) { put(1); get(1); sum += total(); }
                 hold[u] = sum;
@@ -938,8 +935,8 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
 
 // ---- the table's gradient from the partials: sums over samples and places first, then by bucket.
 // BLOCKS.  by_block (H, classes, 64): a class is (row difference, column-group difference) of a block's query and key groups, G =
-// columns / 32 groups a row (a single row: G = all of them).  grid (classes, H), 16 row lanes x 64 places.
-__global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float* by_block, int q_row0, int q_rows, int k_rows, int gq, int gk) {
+// columns / 32 groups a row (a single row: G = all of them).  grid (classes, H), 16 row lanes x 64 places; `more`: samples behind those that are summed already.
+__global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float* by_block, bool more, int q_rows, int k_rows, int gq, int gk) {
     __shared__ float red[1024];
     const int cls = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, r = threadIdx.x >> 6;
     const int dgs = gq + gk - 1;
@@ -972,7 +969,8 @@ __global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float
     __syncthreads();
     if (r == 0) {
         for (int k = 1; k < 16; ++k) s += red[k * 64 + lane];
-        by_block[((int64_t)h * gridDim.x + cls) * 64 + lane] = s;
+        float* o = by_block + ((int64_t)h * gridDim.x + cls) * 64 + lane;
+        *o = more ? *o + s : s;
     }
 }
 
@@ -1003,7 +1001,7 @@ __global__ __launch_bounds__(256) void attn_block_bucket_kernel(AttnArgs a, cons
 }
 
 // DIAGONALS.  by_dist (H, 2, n_dist): grid (distances / 64, 2 classes x H), 16 row lanes x 64 distances.
-__global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_dist, int n_dist, int d0) {
+__global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_dist, bool more, int n_dist, int d0) {
     __shared__ float red[1024];
     const int i = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
     const int cls = blockIdx.y & 1, h = blockIdx.y >> 1, dist = i + d0;
@@ -1019,7 +1017,8 @@ __global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_d
     __syncthreads();
     if (r == 0 && i < n_dist) {
         for (int k = 1; k < 16; ++k) s += red[k * 64 + (threadIdx.x & 63)];
-        by_dist[((int64_t)h * 2 + cls) * n_dist + i] = s;
+        float* o = by_dist + ((int64_t)h * 2 + cls) * n_dist + i;
+        *o = more ? *o + s : s;
     }
 }
 
@@ -1270,7 +1269,9 @@ int check_desc(const rgbd_attn_desc* d, const char* who) {
     RGBD_REQUIRE(d->D == 32 || d->D == 64 || d->D == 128, "%s: head size %d is not one of 32, 64, 128", who, d->D);
     RGBD_REQUIRE(d->Lq < (1 << 24) && d->Lk < (1 << 24) && (int64_t)d->B * d->H * (ceil_div(d->Lq, BLK) + ceil_div(d->Lk, BLK)) < (1 << 30),
                  "%s: too many tokens", who);
-    RGBD_REQUIRE(d->cap >= 0.f, "%s: cap must not be negative", who);
+    // (the kernels divide by both)
+    RGBD_REQUIRE(d->cap == 0.f || (d->cap >= 1e-30f && d->cap <= 1e30f), "%s: cap must be 0 or in [1e-30, 1e30], got %g", who, d->cap);
+    RGBD_REQUIRE(fabsf(d->scale) >= 1e-30f && fabsf(d->scale) <= 1e30f, "%s: |scale| must lie in [1e-30, 1e30], got %g", who, d->scale);
     const int64_t st[9] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh};
     for (int i = 0; i < 9; ++i) RGBD_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
     for (int i = 1; i < 9; i += 3) RGBD_REQUIRE(st[i] >= 0 && st[i] < (1 << 24), "%s: token strides must lie in [0, 2^24) elements", who);
@@ -1349,7 +1350,8 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
     return 0;
 }
 
-// Floats of the backward workspace: delta, the partials and what the first reduction leaves of them.
+constexpr int64_t PART_FLOATS = 128 << 20;
+// Floats of the backward workspace: delta, the partials of `chunk` samples and what the first reduction leaves of them.
 // Few (query, head) pairs over many keys: the number of runs the keys are cut into, 0 for the other form.  Both read a key block once a
 // workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.
 int few_splits(const rgbd_attn_desc* d) {
@@ -1382,9 +1384,10 @@ int kv_splits(const rgbd_attn_desc* d) {
     return (int)(s < 1 ? 1 : s);
 }
 
-struct BwdSizes { int64_t delta, part, sums, kv; int mode, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
+struct BwdSizes { int64_t delta, part, sums, kv; int mode, chunk, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
 BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};
+    z.chunk = d->B;
     z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
     const int ks = kv_splits(d);
     z.kv = ks > 1 ? (int64_t)ks * d->B * d->Hkv * d->Lk * 2 * d->D : 0;
@@ -1392,7 +1395,7 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     const int KT = kt_dq(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
         z.mode = DT_BLOCKS;
-        z.part = (int64_t)d->B * d->H * n_qb * 4 * n_kt * (KT / 32) * 64;
+        z.part = (int64_t)d->H * n_qb * 4 * n_kt * (KT / 32) * 64;
         z.gq = d->rows == 1 ? n_qb * 4 : d->cols / 32;
         z.gk = d->rows == 1 ? n_kt * (KT / 32) : d->cols / 32;
         z.q_row0 = d->rows == 1 ? 0 : d->q_start / d->cols;
@@ -1402,11 +1405,15 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     } else {
         z.mode = DT_DIAGONALS;
         z.span = n_kt * KT + BLK;
-        z.part = (int64_t)d->B * d->H * n_qb * 2 * z.span;
+        z.part = (int64_t)d->H * n_qb * 2 * z.span;
         z.d0 = d->q_start - (n_kt * KT - 1);                          // distances from there to q_start + n_qb * BLK - 1
         z.n_dist = d->q_start + n_qb * BLK - z.d0;
         z.sums = (int64_t)d->H * 2 * z.n_dist;
     }
+    // (a 64 x 64 map's partials are 4 MB a sample and head; from 512 MB on dq runs over as many samples at a time as stay below)
+    z.chunk = (int)((PART_FLOATS + z.part - 1) / z.part);
+    if (z.chunk > d->B) z.chunk = d->B;
+    z.part *= z.chunk;
     z.sums = (z.sums + 3) / 4 * 4;
     return z;
 }
@@ -1502,22 +1509,33 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
         a.seg_tiles = w.tiles;
         a.win_bytes = w.win_bytes;
         const size_t lds = 4 * a.kt * 2 * d->D + dt_lds(z.mode, d->D) + w.lds;
-        const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
-        const int rc = d->D == 32 ? launch_dq<32>(a, bias, cap, z.mode, grid, lds, s) : d->D == 64 ? launch_dq<64>(a, bias, cap, z.mode, grid, lds, s)
-                                                                                               : launch_dq<128>(a, bias, cap, z.mode, grid, lds, s);
-        if (rc) return rc;
-        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dq)");
+        for (int b0 = 0; b0 < d->B; b0 += z.chunk) {
+            AttnArgs c = a;
+            c.B = d->B - b0 < z.chunk ? d->B - b0 : z.chunk;
+            const int64_t rows = (int64_t)b0 * a.H * a.Lq;
+            c.q += b0 * a.q_sb; c.k += b0 * a.k_sb; c.v += b0 * a.v_sb; c.dq += b0 * a.dq_sb;
+            c.d_o += rows * d->D; c.o += rows * d->D; c.o_lo += rows * d->D;
+            c.lse += rows; c.delta += rows;
+            if (c.lengths) c.lengths += b0;
+            const unsigned grid = (unsigned)c.B * a.H * a.n_qb;
+            const int rc = d->D == 32   ? launch_dq<32>(c, bias, cap, z.mode, grid, lds, s)
+                           : d->D == 64 ? launch_dq<64>(c, bias, cap, z.mode, grid, lds, s)
+                                        : launch_dq<128>(c, bias, cap, z.mode, grid, lds, s);
+            if (rc) return rc;
+            RGBD_CHECK_LAUNCH("rgbd_attention_bwd (dq)");
+            if (z.mode == DT_BLOCKS)
+                hipLaunchKernelGGL(attn_block_sums_kernel, dim3((z.q_rows + z.k_rows - 1) * (z.gq + z.gk - 1), a.H), dim3(1024), 0, s, c, sums,
+                                   b0 > 0, z.q_rows, z.k_rows, z.gq, z.gk);
+            else if (z.mode == DT_DIAGONALS)
+                hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 64), 2 * a.H), dim3(1024), 0, s, c, sums, b0 > 0, z.n_dist, z.d0);
+        }
+        if (z.mode == DT_BLOCKS)
+            hipLaunchKernelGGL(attn_block_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.q_row0, z.k_rows,
+                               z.q_rows, z.gq, z.gk);
+        else if (z.mode == DT_DIAGONALS)
+            hipLaunchKernelGGL(attn_dist_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.n_dist, z.d0);
+        RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
     }
-    if (z.mode == DT_BLOCKS) {
-        const int classes = (z.q_rows + z.k_rows - 1) * (z.gq + z.gk - 1);
-        hipLaunchKernelGGL(attn_block_sums_kernel, dim3(classes, a.H), dim3(1024), 0, s, a, sums, z.q_row0, z.q_rows, z.k_rows, z.gq, z.gk);
-        hipLaunchKernelGGL(attn_block_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.q_row0, z.k_rows,
-                           z.q_rows, z.gq, z.gk);
-    } else if (z.mode == DT_DIAGONALS) {
-        hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 64), 2 * a.H), dim3(1024), 0, s, a, sums, z.n_dist, z.d0);
-        hipLaunchKernelGGL(attn_dist_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.n_dist, z.d0);
-    }
-    if (z.mode) RGBD_CHECK_LAUNCH("rgbd_attention_bwd (table)");
     if (d->Lk > 0) {
         const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
         a.kt = kt_of(d->D);

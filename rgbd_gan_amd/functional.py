@@ -1752,7 +1752,7 @@ class _Attention(torch.autograd.Function):
         q, k, v, table, lengths, *kept = ctx.saved_tensors
         grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
         of = kernels.AttnOperands.of
-        dtable = kernels.attention_bwd(of(q, k, v), of(*grads), d_o.contiguous(), *kept, table, ctx.buckets, lengths, *ctx.spec,
+        dtable = kernels.attention_bwd(of(q, k, v), of(*grads), _aligned(d_o), *kept, table, ctx.buckets, lengths, *ctx.spec,
                                        want_table=ctx.needs_input_grad[3])
         return *grads, dtable, None, None, None
 
@@ -1774,9 +1774,15 @@ class _AttentionPacked(torch.autograd.Function):
         qkv, table, lengths, *kept = ctx.saved_tensors
         dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         of = kernels.AttnOperands.packed
-        dtable = kernels.attention_bwd(of(qkv, *ctx.heads), of(dqkv, *ctx.heads), d_o.contiguous(), *kept, table, ctx.buckets, lengths,
+        dtable = kernels.attention_bwd(of(qkv, *ctx.heads), of(dqkv, *ctx.heads), _aligned(d_o), *kept, table, ctx.buckets, lengths,
                                        *ctx.spec, want_table=ctx.needs_input_grad[1])
         return dqkv, dtable, None, None, None, None
+
+
+def _aligned(t):
+    """t contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def _readable(t):
@@ -1791,7 +1797,8 @@ def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=No
     q (B, Lq, H, D), k, v (B, Lk, Hkv, D) bf16 at any strides, D 32, 64 or 128, H a multiple of Hkv (query head h reads key / value
     head h // (H // Hkv)); scale defaults to D ** -0.5, cap 0 leaves scores uncapped; lengths (B,) int32 on the device.
     table (H, n_buckets) fp32 with `buckets` (RelativeBuckets): the bias table[h, bucket of the offset], query i at token
-    q_start + i of the grid, key j at token j.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table."""
+    q_start + i of the grid, key j at token j; values at or below -1e30 (and -inf) leave their offsets out.  A grid of more than one
+    row has at most 1024 columns.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table."""
     spec = (None if scale is None else float(scale), float(cap or 0.0), int(q_start))
     q, k, v = _readable(q), _readable(k), _readable(v)
     table = table.contiguous() if table is not None else None

@@ -1698,8 +1698,10 @@ def _attn_desc(op, table, buckets, lengths, scale, cap, q_start, lse=0, fine=0):
     B, H, Hkv, Lq, Lk, D = op.sizes
     if H < 1 or Hkv < 1 or H % Hkv:
         raise RuntimeError(f"attention: {Hkv} key / value heads do not divide {H} query heads")
-    if not cap >= 0:
-        raise RuntimeError(f"attention: cap must not be negative, got {cap}")
+    if not (cap == 0 or 1e-30 <= cap <= 1e30):
+        raise RuntimeError(f"attention: cap must be 0 or in [1e-30, 1e30], got {cap}")
+    if not 1e-30 <= abs(scale) <= 1e30:
+        raise RuntimeError(f"attention: |scale| must lie in [1e-30, 1e30], got {scale}")
     rows = cols = n_buckets = tab = bmap = lens = 0
     if (table is None) != (buckets is None):
         raise RuntimeError("attention: a bias table and its buckets come together")

@@ -75,6 +75,11 @@ def test_attention_refuses_what_it_cannot_compute():
         (dict(k=bf(2, 9, 3, 64), v=bf(2, 9, 3, 64)), "do not divide"),
         (dict(cap=-1.0), "cap"),
         (dict(cap=float("nan")), "cap"),
+        (dict(cap=float("inf")), "cap"),
+        (dict(cap=1e-35), "cap"),
+        (dict(scale=0.0), "scale"),
+        (dict(scale=float("nan")), "scale"),
+        (dict(scale=float("inf")), "scale"),
         (dict(table=table), "come together"),
         (dict(buckets=b), "come together"),
         (dict(table=table[:3], buckets=b), "table must be"),
@@ -129,10 +134,11 @@ def test_c_entries_report_bad_arguments():
     assert lib.rgbd_group_norm_bwd(16, 8, 16, 16, 16, 16, 16, 16, 16, 16, 2, 16, 2048, 4, 0, 0, 0.2, None) == -1
     assert lib.rgbd_attention_fwd(None, None, None, None, None) == -1
     d = kernels._AttnDesc()
-    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D = 1, 2, 1, 4, 4, 64
+    d.B, d.H, d.Hkv, d.Lq, d.Lk, d.D, d.scale = 1, 2, 1, 4, 4, 64, 0.125
     ok = lambda: lib.rgbd_attention_bwd_workspace(ctypes.byref(d), 0)
     assert ok() > 0
-    for name, value in (("D", 40), ("Hkv", 3), ("H", 0), ("Lq", -1), ("cap", -1.0), ("q_sl", 4), ("k", 8)):
+    for name, value in (("D", 40), ("Hkv", 3), ("H", 0), ("Lq", -1), ("cap", -1.0), ("cap", float("nan")), ("scale", 0.0), ("q_sl", 4), ("k_sl", 1 << 24),
+                        ("v_sl", -64), ("k", 8)):
         old = getattr(d, name)
         setattr(d, name, value)
         assert ok() == -1, name

@@ -191,20 +191,72 @@ def test_minus_infinity_in_the_table_masks_offsets():
     m[:, cols - 1:] = 1                                           # dx >= 0
     b = RelativeBuckets(m, 2, device=DEV)
     q, k, v, _, do = inputs(5, 2, 66, 66, 2, 2, 32)
-    for low in (-math.inf, torch.finfo(torch.float32).min):
-        table = torch.tensor([[low, 0.5], [0.25, low]], device=DEV)
-        args = (q, k, v, table, b, do)
-        got = run(*args)
-        if low == -math.inf:
-            want = definition(*args, None, 0.0, None, 0, True)
-            check(got, want, ["o", "dq", "dk", "dv", "dtable"])
-            assert float(got["dtable"][0, 0]) == 0.0 and float(got["dtable"][1, 1]) == 0.0
+    want = definition(q, k, v, torch.tensor([[-math.inf, 0.5], [0.25, -math.inf]], device=DEV), b, do, None, 0.0, None, 0, True)
+    for low in (-math.inf, torch.finfo(torch.float32).min, -1e30):
+        got = run(q, k, v, torch.tensor([[low, 0.5], [0.25, low]], device=DEV), b, do)
+        check(got, want, ["o", "dq", "dk", "dv", "dtable"])
+        assert float(got["dtable"][0, 0]) == 0.0 and float(got["dtable"][1, 1]) == 0.0
         # head 1 sees only keys to its right: the last column has none
-        last = got["o"].reshape(2, rows, cols, 2, 32)[:, :, -1, 1].float()
-        if low == -math.inf:
-            assert float(last.abs().max()) == 0.0
-        else:                                                     # finite: an empty row is an average over its own lowest scores
-            assert torch.isfinite(last).all()
+        assert float(got["o"].reshape(2, rows, cols, 2, 32)[:, :, -1, 1].float().abs().max()) == 0.0
+    # one query row of it, over enough keys for the form that cuts them into runs
+    m = torch.zeros(1, 1199, dtype=torch.long)
+    m[:, 599:] = 1
+    b = RelativeBuckets(m, 2, device=DEV)
+    q, k, v, _, do = inputs(5, 2, 2, 600, 2, 2, 32)
+    want = definition(q, k, v, torch.tensor([[-math.inf, 0.5], [0.25, -math.inf]], device=DEV), b, do, None, 0.0, None, 0, True)
+    for low in (-math.inf, torch.finfo(torch.float32).min):
+        check(run(q, k, v, torch.tensor([[low, 0.5], [0.25, low]], device=DEV), b, do), want, ["o", "dq", "dk", "dv", "dtable"])
+
+
+def test_a_bias_far_from_zero():
+    """Every score of a head moved by -3000, by +3000, by +-80: the softmax does not care, its reference has to follow."""
+    b = buckets(9, 9, 7)
+    q, k, v, table, do = inputs(25, 2, 81, 81, 4, 2, 64, b.n_buckets)
+    shift = torch.tensor([-3000.0, 3000.0, -80.0, 80.0], device=DEV)[:, None]
+    full_check(q, k, v, table + shift, b, do)
+    full_check(q, k, v, table + shift, b, do, cap=9.0, lengths=torch.tensor([81, 33], dtype=torch.int32, device=DEV))
+
+
+def test_scores_that_grow_and_fall_along_the_keys():
+    """Scores that leave the range of the running reference in either direction, in the middle of the keys and at their end."""
+    N = 400
+    for sign in (1.0, -1.0):
+        g = torch.Generator(device=DEV).manual_seed(26)
+        r = lambda *s: torch.randn(*s, generator=g, device=DEV)
+        q, k, v, do = (r(1, N, 1, 64) for _ in range(4))
+        k = k + sign * torch.linspace(-12, 12, N, device=DEV)[None, :, None, None] * (torch.arange(64, device=DEV) == 3)
+        q = q + 20.0 * (torch.arange(64, device=DEV) == 3)
+        full_check(*(t.to(BF16) for t in (q, k, v)), None, None, do.to(BF16), scale=0.5)
+
+
+def test_ties_between_bf16_neighbours():
+    """o halfway between two bf16 numbers, everywhere and of either parity: its low half has to tell on which side the rounding went, or
+    delta, and with it every gradient, is off by a whole step of o."""
+    b = buckets(1, 2, 3)
+    g = torch.Generator(device=DEV).manual_seed(27)
+    v0 = torch.randn(3, 2, 64, generator=g, device=DEV).to(BF16)
+    v1 = (v0.view(torch.int16) + 1).view(BF16)                          # the next one away from zero
+    v = torch.stack([v0, v1], dim=1)
+    q, k = torch.zeros(3, 2, 2, 64, device=DEV, dtype=BF16), torch.randn(3, 2, 2, 64, generator=g, device=DEV).to(BF16)
+    do = torch.randn(3, 2, 2, 64, generator=g, device=DEV).to(BF16)
+    table = torch.zeros(2, b.n_buckets, device=DEV)
+    full_check(q, k, v, table, b, do)
+
+
+def test_a_batch_whose_partials_are_reduced_in_pieces():
+    """The table's gradient of a batch large enough for its partial sums to be reduced a few samples at a time: the other gradients
+    are those of its halves bit for bit, dtable is their sum up to the order of fp32 additions."""
+    for rows, cols, B, H in ((64, 64, 18, 8), (63, 65, 17, 32)):
+        b = buckets(rows, cols, 7)
+        q, k, v, table, do = inputs(28, B, rows * cols, rows * cols, H, H, 32, b.n_buckets)
+        lengths = torch.randint(1, rows * cols, (B,), dtype=torch.int32, device=DEV)
+        whole = run(q, k, v, table, b, do, lengths=lengths)
+        h = B // 2
+        parts = [run(*(t[s] for t in (q, k, v)), table, b, do[s], lengths=lengths[s]) for s in (slice(0, h), slice(h, B))]
+        for n in ("o", "dq", "dk", "dv"):
+            assert torch.equal(whole[n], torch.cat([x[n] for x in parts])), (rows, n)
+        both = parts[0]["dtable"].double() + parts[1]["dtable"].double()
+        assert float((whole["dtable"].double() - both).norm() / both.norm()) <= 2.0 ** -18
 
 
 def test_strides_orders_and_packed_layouts():
@@ -234,6 +286,14 @@ def test_strides_orders_and_packed_layouts():
         want = torch.cat([base[n].flatten(2) for n in ("dq", "dk", "dv")], dim=-1).reshape(shape)
         assert torch.equal(dqkv, want)
         assert torch.equal(Fn.attention_packed(qkv.detach(), H, Hkv, table, b), base["plain"])
+    # an output gradient at an odd address, and one that is a single number for all
+    buf = torch.empty(do.numel() + 8, dtype=BF16, device=DEV)
+    odd_do = buf[5:5 + do.numel()].view(do.shape)
+    odd_do.copy_(do)
+    got = run(q, k, v, table, b, odd_do)
+    assert all(torch.equal(base[n], got[n]) for n in base)
+    got, ones = run(q, k, v, table, b, torch.ones(1, 1, 1, 1, dtype=BF16, device=DEV).expand(do.shape)), run(q, k, v, table, b, torch.ones_like(do))
+    assert all(torch.equal(ones[n], got[n]) for n in ones)
     # one k, v for the whole batch (stride 0) and its summed gradient
     k1, v1 = (t[:1].clone().requires_grad_(True) for t in (k, v))
     # (a table that is learned: its gradient asks for the finer second product, as in run())
