@@ -1275,11 +1275,12 @@ int check_desc(const rgbd_attn_desc* d, const char* who) {
     RGBD_REQUIRE(d->B >= 0 && d->H > 0 && d->Hkv > 0 && d->Lq >= 0 && d->Lk >= 0 && d->H % d->Hkv == 0,
                  "%s: bad sizes B=%d H=%d Hkv=%d Lq=%d Lk=%d (Hkv must divide H)", who, d->B, d->H, d->Hkv, d->Lq, d->Lk);
     RGBD_REQUIRE(d->D == 32 || d->D == 64 || d->D == 128, "%s: head size %d is not one of 32, 64, 128", who, d->D);
-    RGBD_REQUIRE(d->Lq < (1 << 24) && d->Lk < (1 << 24) && (int64_t)d->B * d->H * (ceil_div(d->Lq, BLK) + ceil_div(d->Lk, BLK)) < (1 << 30),
-                 "%s: too many tokens", who);
-    // (the kernels divide by both)
-    RGBD_REQUIRE(d->cap == 0.f || (d->cap >= 1e-30f && d->cap <= 1e30f), "%s: cap must be 0 or in [1e-30, 1e30], got %g", who, d->cap);
-    RGBD_REQUIRE(fabsf(d->scale) >= 1e-30f && fabsf(d->scale) <= 1e30f, "%s: |scale| must lie in [1e-30, 1e30], got %g", who, d->scale);
+    // (a launch has fewer than 2^32 threads)
+    RGBD_REQUIRE(d->Lq < (1 << 24) && d->Lk < (1 << 24) && (int64_t)d->H * d->D < (1 << 24) &&
+                 (int64_t)d->B * d->H * (ceil_div(d->Lq, BLK) + ceil_div(d->Lk, BLK)) < (1 << 23), "%s: too many heads or tokens", who);
+    // (the kernels divide by both, and by their quotient)
+    RGBD_REQUIRE(d->cap == 0.f || (d->cap >= 1e-12f && d->cap <= 1e12f), "%s: cap must be 0 or in [1e-12, 1e12], got %g", who, d->cap);
+    RGBD_REQUIRE(fabsf(d->scale) >= 1e-12f && fabsf(d->scale) <= 1e12f, "%s: |scale| must lie in [1e-12, 1e12], got %g", who, d->scale);
     const int64_t st[9] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh};
     for (int i = 0; i < 9; ++i) RGBD_REQUIRE(st[i] % 8 == 0, "%s: strides must be multiples of 8 elements", who);
     for (int i = 1; i < 9; i += 3) RGBD_REQUIRE(st[i] >= 0 && st[i] < (1 << 24), "%s: token strides must lie in [0, 2^24) elements", who);
@@ -1358,12 +1359,10 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
     return 0;
 }
 
-constexpr int64_t PART_FLOATS = 128 << 20;
-// Floats of the backward workspace: delta, the partials of `chunk` samples and what the first reduction leaves of them.
 // Few (query, head) pairs over many keys: the number of runs the keys are cut into, 0 for the other form.  Both read a key block once a
 // workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.
 int few_splits(const rgbd_attn_desc* d) {
-    if ((int64_t)d->H / d->Hkv * d->Lq > 32 || d->Lk <= 256) return 0;
+    if ((int64_t)d->H / d->Hkv * d->Lq > 32 || d->Lk <= 256 || (int64_t)d->B * d->H * d->Lq >= 1 << 20) return 0;
     const int64_t groups = (int64_t)d->B * d->Hkv, want = d->D == 128 ? 256 : 512;   // workgroups that fit the chip at once (LDS)
     int64_t s = (want + groups - 1) / groups;
     const int64_t most = ceil_div(d->Lk, 32 * 8);                     // two blocks for every wave
@@ -1392,6 +1391,9 @@ int kv_splits(const rgbd_attn_desc* d) {
     return (int)(s < 1 ? 1 : s);
 }
 
+// Floats of the backward workspace: delta, the table's partials of `chunk` samples (PART_FLOATS at most, or one sample), what the first
+// reduction leaves of them, the runs' dk and dv.
+constexpr int64_t PART_FLOATS = 128 << 20;
 struct BwdSizes { int64_t delta, part, sums, kv; int mode, chunk, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
 BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};

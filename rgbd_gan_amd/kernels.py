@@ -1651,7 +1651,7 @@ class AttnOperands:
 
     @staticmethod
     def readable(t, strides):
-        return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in strides)
+        return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and strides[1] < 1 << 24 and not any(s % 8 for s in strides)
 
     @classmethod
     def of(cls, q, k, v):
@@ -1670,7 +1670,7 @@ class AttnOperands:
         for t, name in ((q, "q"), (k, "k"), (v, "v")):
             st = cls._axis(t)
             if not cls.readable(t, st):
-                raise RuntimeError(f"attention: {name}: head vectors must be contiguous, strides multiples of 8, 16-byte aligned")
+                raise RuntimeError(f"attention: {name}: head vectors must be contiguous, 16-byte aligned, strides multiples of 8, a token's below 2^24")
             op.ptrs.append(t.data_ptr())
             op.strides += st
         return op
@@ -1686,7 +1686,7 @@ class AttnOperands:
         op = cls()
         sb, sl = cls._axis(qkv, 2)
         if not cls.readable(qkv, (sb, sl)):
-            raise RuntimeError("attention: qkv: a token's channels must be contiguous, strides multiples of 8, 16-byte aligned")
+            raise RuntimeError("attention: qkv: a token's channels must be contiguous, 16-byte aligned, strides multiples of 8, a token's below 2^24")
         p = qkv.data_ptr()
         op.sizes, op.tensors = (B, heads, kv_heads, N, N, D), (qkv,)
         op.ptrs = [p, p + 2 * heads * D, p + 2 * (heads + kv_heads) * D] if p else [0, 0, 0]
@@ -1698,10 +1698,10 @@ def _attn_desc(op, table, buckets, lengths, scale, cap, q_start, lse=0, fine=0):
     B, H, Hkv, Lq, Lk, D = op.sizes
     if H < 1 or Hkv < 1 or H % Hkv:
         raise RuntimeError(f"attention: {Hkv} key / value heads do not divide {H} query heads")
-    if not (cap == 0 or 1e-30 <= cap <= 1e30):
-        raise RuntimeError(f"attention: cap must be 0 or in [1e-30, 1e30], got {cap}")
-    if not 1e-30 <= abs(scale) <= 1e30:
-        raise RuntimeError(f"attention: |scale| must lie in [1e-30, 1e30], got {scale}")
+    if not (cap == 0 or 1e-12 <= cap <= 1e12):
+        raise RuntimeError(f"attention: cap must be 0 or in [1e-12, 1e12], got {cap}")
+    if not 1e-12 <= abs(scale) <= 1e12:
+        raise RuntimeError(f"attention: |scale| must lie in [1e-12, 1e12], got {scale}")
     rows = cols = n_buckets = tab = bmap = lens = 0
     if (table is None) != (buckets is None):
         raise RuntimeError("attention: a bias table and its buckets come together")
@@ -1748,7 +1748,7 @@ def _attn_workspace(op, buckets, q_start, kind, ask):
 
 def attention_fwd(op, table=None, buckets=None, lengths=None, scale=None, cap=0.0, q_start=0, keep=False, fine=False):
     """op: AttnOperands -> o (B, Lq, H, D) bf16 and, with `keep`, what the backward pass needs: o_lo (the low 16 bits of o's fp32 values, typed bf16) and
-    lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient needs of o (probabilities with 16 bits in the second product)."""
+    lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient needs of o (probabilities with 24 bits in the second product)."""
     B, H, Hkv, Lq, Lk, D = op.sizes
     t = op.tensors[0]
     o = torch.empty((B, Lq, H, D), dtype=BF16, device=t.device)

@@ -77,6 +77,7 @@ def test_attention_refuses_what_it_cannot_compute():
         (dict(cap=float("nan")), "cap"),
         (dict(cap=float("inf")), "cap"),
         (dict(cap=1e-35), "cap"),
+        (dict(cap=1e13), "cap"),
         (dict(scale=0.0), "scale"),
         (dict(scale=float("nan")), "scale"),
         (dict(scale=float("inf")), "scale"),
@@ -138,7 +139,7 @@ def test_c_entries_report_bad_arguments():
     ok = lambda: lib.rgbd_attention_bwd_workspace(ctypes.byref(d), 0)
     assert ok() > 0
     for name, value in (("D", 40), ("Hkv", 3), ("H", 0), ("Lq", -1), ("cap", -1.0), ("cap", float("nan")), ("scale", 0.0), ("q_sl", 4), ("k_sl", 1 << 24),
-                        ("v_sl", -64), ("k", 8)):
+                        ("v_sl", -64), ("k", 8), ("B", 1 << 22), ("scale", 1e13)):
         old = getattr(d, name)
         setattr(d, name, value)
         assert ok() == -1, name

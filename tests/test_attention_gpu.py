@@ -380,6 +380,82 @@ def test_captured_graphs_replay_with_new_inputs():
             assert all(torch.equal(x, y) for x, y in zip(again, eager[j]))
 
 
+def test_other_forms_captured_and_replayed():
+    """The forms that the sizes above do not reach: keys in runs (few queries), queries in runs (few keys), offsets by diagonals and by
+    blocks, a table without gradient; each captured, replayed with new inputs, the eager pass in between."""
+    from rgbd_gan_amd import functional as Fn
+    for rows, cols, lq, H, Hkv, D, learned in ((1, 1400, 3, 4, 1, 64, True), (33, 20, 0, 8, 2, 32, True), (32, 32, 0, 1, 1, 128, True),
+                                              (16, 20, 0, 2, 2, 64, False)):
+        n = rows * cols
+        lq = lq or n
+        b = buckets(rows, cols, 7)
+        sets = [inputs(40 + i, 2, lq, n, H, Hkv, D, b.n_buckets) for i in range(3)]
+        lens = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ([n, 60], [0, n], [n - 1, 1])]
+
+        def passes(q, k, v, table, do, lengths):
+            leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+            table = table.detach().requires_grad_(learned)
+            o = Fn.attention(*leaves, table, b, lengths=lengths, q_start=n - lq)
+            return (o.detach(), *torch.autograd.grad(o, leaves + [table] * learned, do))
+
+        eager = [passes(*s, l) for s, l in zip(sets, lens)]
+        hold = [t.clone() for t in sets[0]] + [lens[0].clone()]
+        st = torch.cuda.Stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            passes(*hold)
+        torch.cuda.current_stream().wait_stream(st)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = passes(*hold)
+        for j in (1, 2, 0, 1):
+            for t, s in zip(hold, list(sets[j]) + [lens[j]]):
+                t.copy_(s)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, eager[j])), (rows, cols, j)
+            assert all(torch.equal(x, y) for x, y in zip(passes(*sets[j], lens[j]), eager[j]))
+
+
+def test_nothing_is_read_that_was_not_written():
+    """Memory that held NaN before a call (workspaces, statistics, outputs) changes nothing."""
+    for rows, cols, lq, lk, B, H, Hkv, D, lens in (
+            (1, 1400, 3, 0, 2, 4, 1, 64, [1400, 9]), (33, 20, 0, 0, 2, 8, 2, 32, [0, 321]), (32, 32, 0, 0, 2, 2, 1, 128, [1024, 70]),
+            (64, 64, 130, 0, 1, 1, 1, 64, [2000]), (1, 300, 0, 0, 3, 2, 2, 64, [300, 1, 0]), (12, 20, 50, 100, 2, 2, 2, 64, [40, 100]),
+            (32, 32, 64, 900, 1, 2, 2, 64, None), (7, 8, 0, 0, 2, 2, 1, 32, [56, 3])):
+        n = rows * cols
+        lq, lk = lq or n, lk or n
+        b = buckets(rows, cols, 7)
+        q, k, v, table, do = inputs(50, B, lq, lk, H, Hkv, D, b.n_buckets)
+        lengths = torch.tensor(lens, dtype=torch.int32, device=DEV) if lens is not None else None
+        args = dict(lengths=lengths, q_start=n - lq)
+        want = definition(q, k, v, table, b, do, None, 0.0, lengths, n - lq, True)
+        for size in (1 << 8, 1 << 14, 1 << 18, 1 << 21, 1 << 23):        # blocks of every pool the allocator gives out again
+            held = [torch.full((size,), math.nan, device=DEV) for _ in range(8)]
+            del held
+        check(run(q, k, v, table, b, do, **args), want, ["o", "dq", "dk", "dv", "dtable"])
+
+
+def test_a_negative_scale_is_a_negative_query():
+    b = buckets(9, 13, 7)
+    q, k, v, table, do = inputs(60, 2, 117, 117, 4, 2, 64, b.n_buckets)
+    for cap in (0.0, 6.0):
+        got = run(q, k, v, table, b, do, scale=-0.3, cap=cap)
+        got["dq"] = -got["dq"]
+        check(got, definition(-q, k, v, table, b, do, 0.3, cap, None, 0, True), ["o", "dq", "dk", "dv", "dtable"])
+
+
+def test_a_table_without_gradient():
+    from rgbd_gan_amd import functional as Fn
+    b = buckets(13, 11, 7)
+    q, k, v, table, do = inputs(61, 2, 143, 143, 2, 1, 64, b.n_buckets)
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+    o = Fn.attention(*leaves, table, b, cap=12.0)
+    got = {"o": o.detach(), **dict(zip(("dq", "dk", "dv"), torch.autograd.grad(o, leaves, do)))}
+    check(got, definition(q, k, v, table, b, do, None, 12.0, None, 0, False), list(got))
+
+
 def test_gradients_against_differences():
     """<gradient, direction> against central differences of the 64-bit definition, h small enough for their own error to vanish
     next to the tolerance summed over the direction."""

@@ -88,6 +88,13 @@ def test_group_norm(shape, groups, dtype):
         check(*inputs(i, shape, dtype), groups, act)
 
 
+@pytest.mark.parametrize("shape,groups,dtype", [((1, 20, 30, 8192), 8192, BF16), ((2, 9, 8192), 1, BF16), ((1, 25, 20, 4096), 4096, F32),
+                                                ((1, 25, 20, 4096), 2, F32), ((2, 31, 7, 1023), 1023, BF16), ((300, 3, 40), 8, F32)],
+                         ids=lambda s: str(s).replace(" ", ""))
+def test_the_widest_maps_and_many_samples(shape, groups, dtype):
+    check(*inputs(9, shape, dtype), groups, "silu")
+
+
 def test_means_far_from_zero_cost_no_digits():
     """|mean| = 1000 spreads: sums of squares would leave nothing of the variance in fp32."""
     for shape in ((2, 16, 16, 32), (1, 128, 128, 32)):
