@@ -533,6 +533,14 @@ template <int D> struct WaveDma {
     }
 };
 
+// Value d of a row from its sums: s over the keys, reference m, probabilities l.
+__device__ __forceinline__ void write_few(const AttnArgs& a, int64_t row, int64_t lse_row, int D, int d, float s, float m, float l) {
+    const float y = l > 0.f ? s / l : (l == 0.f ? 0.f : l);           // no key: 0; a NaN stays one
+    a.out[row * D + d] = f32_to_bf16_bits(y);
+    if (a.out_lo) a.out_lo[row * D + d] = (unsigned short)low_half(y);
+    if (a.lse && d == 0) a.lse[lse_row] = l == 0.f ? 0.f : m + __builtin_amdgcn_logf(l);
+}
+
 template <int D, bool BIAS, bool CAP>
 __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -658,7 +666,7 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
         for (int i = 0; i < 16; ++i) jo[(wave * 32 + col) * (D + 1) + 32 * d + 8 * (i >> 2) + 4 * half + (i & 3)] = o[d][i];
     if (half == 0) { jm[wave * 64 + col] = m; jm[wave * 64 + 32 + col] = l; }
     __syncthreads();
-    float* part = a.part + (int64_t)blockIdx.x * 32 * (D + 2);
+    float* part = a.splits > 1 ? a.part + (int64_t)blockIdx.x * 32 * (D + 2) : nullptr;
     for (int e = threadIdx.x; e < cols * D; e += 256) {
         const int c = e / D, d = e % D;
         float mm = NEG_INF, s = 0.f, ll = 0.f;
@@ -670,8 +678,13 @@ __global__ __launch_bounds__(256, 1) void attn_few_kernel(AttnArgs a) {
             s += jo[(w * 32 + c) * (D + 1) + d] * al;
             ll += jm[w * 64 + 32 + c] * al;
         }
-        part[c * (D + 2) + d] = s;
-        if (d == 0) { part[c * (D + 2) + D] = mm; part[c * (D + 2) + D + 1] = ll; }
+        if (part) {
+            part[c * (D + 2) + d] = s;
+            if (d == 0) { part[c * (D + 2) + D] = mm; part[c * (D + 2) + D + 1] = ll; }
+        } else {                                                     // one run: the rows are whole
+            const int hc = hk * a.rep + c / a.Lq, qc = c % a.Lq;
+            write_few(a, ((int64_t)b * a.Lq + qc) * a.H + hc, ((int64_t)b * a.H + hc) * a.Lq + qc, D, d, s, mm, ll);
+        }
     }
 }
 
@@ -711,11 +724,7 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
     __syncthreads();
     if (r) return;
     for (int k = 1; k < R; ++k) s += red[k * D + d];
-    const float l = row_l, y = l > 0.f ? s / l : (l == 0.f ? 0.f : l);
-    const int64_t at = (int64_t)blockIdx.x * D + d;
-    a.out[at] = f32_to_bf16_bits(y);
-    if (a.out_lo) a.out_lo[at] = (unsigned short)low_half(y);
-    if (a.lse && d == 0) a.lse[((int64_t)b * a.H + h) * a.Lq + qi] = l == 0.f ? 0.f : row_m + __builtin_amdgcn_logf(l);
+    write_few(a, blockIdx.x, ((int64_t)b * a.H + h) * a.Lq + qi, D, d, s, row_m, row_l);
 }
 
 // ======================================================================================================= dq, delta and the table
@@ -1360,7 +1369,9 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
 }
 
 // Few (query, head) pairs over many keys: the number of runs the keys are cut into, 0 for the other form.  Both read a key block once a
-// workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.
+// workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.  us for
+// one query, 4 samples, 8 query heads on 2 of 64, this form / the other: 256 keys 9 / 6, 512 keys 9 / 10, 1024 keys 9 / 17; 64 samples of 512
+// keys 10 / 15; 4 queries, 256 samples of 1024 keys (one run) 26 / 67; 4 samples of 16384 keys, 8 on 2 of 128: 25 / 563.
 int few_splits(const rgbd_attn_desc* d) {
     if ((int64_t)d->H / d->Hkv * d->Lq > 32 || d->Lk <= 256 || (int64_t)d->B * d->H * d->Lq >= 1 << 20) return 0;
     const int64_t groups = (int64_t)d->B * d->Hkv, want = d->D == 128 ? 256 : 512;   // workgroups that fit the chip at once (LDS)
@@ -1375,20 +1386,23 @@ template <int D> int launch_few(const AttnArgs& a, bool bias, bool cap, hipStrea
     const size_t lds = 4 * 4 * 32 * 2 * D > 4 * (4 * 32 * (D + 1) + 256) ? 4 * 4 * 32 * 2 * D : 4 * (4 * 32 * (D + 1) + 256);
     if (bias) { if (cap) LAUNCH((attn_few_kernel<D, true, true>)); else LAUNCH((attn_few_kernel<D, true, false>)); }
     else { if (cap) LAUNCH((attn_few_kernel<D, false, true>)); else LAUNCH((attn_few_kernel<D, false, false>)); }
-    hipLaunchKernelGGL((attn_few_join_kernel<D>), dim3(a.B * a.H * a.Lq), dim3(512), 0, s, a);
+    if (a.splits > 1) hipLaunchKernelGGL((attn_few_join_kernel<D>), dim3(a.B * a.H * a.Lq), dim3(512), 0, s, a);
     return 0;
 }
 
 // Runs of query tiles for dk, dv: as many as fill the chip once (one workgroup a compute unit at head size 128, two at 64, three at 32:
-// registers), of at least four tiles each.
+// registers), of at least eight tiles each.  The runs' sums are written and read once more in fp32, which two runs of small heads do
+// not earn back.  us cut / whole, the second launch included: 8 x 1024, 8 query heads on 2 of 64 (4 runs) 50 / 86; 1 x 2048, 4 on 2 of 64
+// (8 runs) 26 / 74; 5 x 713, 6 on 2 of 32 (4 runs) 19 / 33; 2 x 4096, 4 on 2 of 128 (4 runs) 220 / 378; 2 x 2048 x 4 of 128 (2 runs) 67 / 94;
+// but 4 x 2048 x 4 of 64 (2 runs) 52 / 47, 12 x 1024 x 4 of 32 (2 runs) 33 / 26, 4 x 1024 x 4 of 64 in 4 runs of 4 tiles 31 / 25.
 int kv_splits(const rgbd_attn_desc* d) {
     const int64_t groups = (int64_t)d->B * d->Hkv * ceil_div(d->Lk, BLK), want = d->D == 128 ? 256 : d->D == 64 ? 512 : 768;
-    if (groups == 0 || groups * 4 > want * 3) return 1;
+    if (groups == 0) return 1;
     int64_t s = want / groups;
-    const int64_t most = (int64_t)d->H / d->Hkv * ceil_div(d->Lq, kt_of(d->D)) / 4;
+    const int64_t most = (int64_t)d->H / d->Hkv * ceil_div(d->Lq, kt_of(d->D)) / 8;
     if (s > most) s = most;
     if (s > 64) s = 64;
-    return (int)(s < 1 ? 1 : s);
+    return s < (d->D == 128 ? 2 : 3) ? 1 : (int)s;
 }
 
 // Floats of the backward workspace: delta, the table's partials of `chunk` samples (PART_FLOATS at most, or one sample), what the first
@@ -1433,7 +1447,8 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
 extern "C" int64_t rgbd_attention_fwd_workspace(const rgbd_attn_desc* d) {
     if (check_desc(d, "rgbd_attention_fwd_workspace")) return -1;
     if (d->B == 0 || d->Lq == 0) return 0;
-    return (int64_t)d->B * d->Hkv * few_splits(d) * 32 * (d->D + 2);
+    const int runs = few_splits(d);
+    return runs > 1 ? (int64_t)d->B * d->Hkv * runs * 32 * (d->D + 2) : 0;
 }
 
 extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, float* workspace, void* stream) {
@@ -1448,7 +1463,7 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
     hipStream_t s = (hipStream_t)stream;
     a.splits = few_splits(d);
     if (a.splits) {
-        RGBD_REQUIRE(workspace != nullptr, "rgbd_attention_fwd: null workspace");
+        RGBD_REQUIRE(workspace || a.splits == 1, "rgbd_attention_fwd: null workspace");
         a.part = workspace;
         const int rc = d->D == 32 ? launch_few<32>(a, d->table, cap, s) : d->D == 64 ? launch_few<64>(a, d->table, cap, s) : launch_few<128>(a, d->table, cap, s);
         if (rc) return rc;

@@ -437,6 +437,19 @@ def test_nothing_is_read_that_was_not_written():
         check(run(q, k, v, table, b, do, **args), want, ["o", "dq", "dk", "dv", "dtable"])
 
 
+def test_many_samples_of_few_queries_and_runs_of_queries():
+    """Enough samples for one run of keys each (the rows are written by the first launch), and shapes on either side of cutting the
+    queries of dk and dv into runs."""
+    b = buckets(20, 21, 7)
+    for B, lq, H, Hkv, D, lens in ((300, 1, 4, 2, 64, None), (260, 3, 8, 1, 32, True), (300, 2, 2, 1, 128, True)):
+        q, k, v, table, do = inputs(70, B, lq, 420, H, Hkv, D, b.n_buckets)
+        lengths = torch.arange(B, dtype=torch.int32, device=DEV) * 3 % 421 if lens else None
+        full_check(q, k, v, table, b, do, lengths=lengths, q_start=11)
+    for B, n, H, Hkv, D in ((2, 700, 6, 2, 32), (1, 520, 16, 1, 64), (1, 513, 4, 1, 128), (1, 500, 4, 4, 64)):
+        q, k, v, _, do = inputs(71, B, n, n, H, Hkv, D)
+        full_check(q, k, v, None, None, do, lengths=torch.tensor([n - 7] * B, dtype=torch.int32, device=DEV))
+
+
 def test_a_negative_scale_is_a_negative_query():
     b = buckets(9, 13, 7)
     q, k, v, table, do = inputs(60, 2, 117, 117, 4, 2, 64, b.n_buckets)
