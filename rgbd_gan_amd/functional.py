@@ -1750,11 +1750,11 @@ class _Attention(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         q, k, v, table, lengths, *kept = ctx.saved_tensors
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v)]
-        of = kernels.AttnOperands.of
-        dtable = kernels.attention_bwd(of(q, k, v), of(*grads), _aligned(d_o), *kept, table, ctx.buckets, lengths, *ctx.spec,
+        op = kernels.AttnOperands.of(q, k, v)
+        grads = op.fresh(op.sizes, q)
+        dtable = kernels.attention_bwd(op, grads, _aligned(d_o), *kept, table, ctx.buckets, lengths, *ctx.spec,
                                        want_table=ctx.needs_input_grad[3])
-        return *grads, dtable, None, None, None
+        return *grads.tensors, dtable, None, None, None
 
 
 class _AttentionPacked(torch.autograd.Function):
@@ -1772,7 +1772,7 @@ class _AttentionPacked(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o):
         qkv, table, lengths, *kept = ctx.saved_tensors
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dqkv = qkv.new_empty(qkv.shape)
         of = kernels.AttnOperands.packed
         dtable = kernels.attention_bwd(of(qkv, *ctx.heads), of(dqkv, *ctx.heads), _aligned(d_o), *kept, table, ctx.buckets, lengths,
                                        *ctx.spec, want_table=ctx.needs_input_grad[1])
@@ -1787,8 +1787,7 @@ def _aligned(t):
 
 def _readable(t):
     """t, or a copy where the kernels cannot read it as it lies (kernels.AttnOperands refuses what is no tensor of theirs at all)."""
-    op = kernels.AttnOperands
-    return t if op.readable(t, op._axis(t, t.dim() - 1)) else t.clone(memory_format=torch.contiguous_format)
+    return t if t.dim() < 3 or kernels.AttnOperands.place(t) is not None else t.clone(memory_format=torch.contiguous_format)
 
 
 def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=None, q_start=0):

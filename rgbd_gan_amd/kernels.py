@@ -1646,12 +1646,16 @@ class AttnOperands:
     __slots__ = ("sizes", "ptrs", "strides", "tensors")
 
     @staticmethod
-    def _axis(t, n_axes=3):
-        return [s if n > 1 else 0 for s, n in zip(t.stride()[:n_axes], t.shape)]
-
-    @staticmethod
-    def readable(t, strides):
-        return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and strides[1] < 1 << 24 and not any(s % 8 for s in strides)
+    def place(t):
+        """Address and strides of t's axes but the last, None where the kernels cannot read it as it lies."""
+        *st, last = t.stride()
+        for i, n in enumerate(t.shape[:-1]):
+            if n <= 1:
+                st[i] = 0
+        p, odd = t.data_ptr(), 0
+        for s in st:
+            odd |= s
+        return None if last != 1 or odd & 7 or p & 15 or st[1] >= 1 << 24 else (p, st)
 
     @classmethod
     def of(cls, q, k, v):
@@ -1665,14 +1669,22 @@ class AttnOperands:
             raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
         if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
             raise RuntimeError(f"attention: k {tuple(k.shape)} / v {tuple(v.shape)} do not match q {tuple(q.shape)}")
+        at = [cls.place(t) for t in (q, k, v)]
+        if None in at:
+            raise RuntimeError(f"attention: {'qkv'[at.index(None)]}: head vectors must be contiguous, 16-byte aligned, strides multiples of 8, "
+                               "a token's below 2^24")
         op = cls()
-        op.sizes, op.tensors, op.ptrs, op.strides = (B, H, k.shape[2], Lq, k.shape[1], D), (q, k, v), [], []
-        for t, name in ((q, "q"), (k, "k"), (v, "v")):
-            st = cls._axis(t)
-            if not cls.readable(t, st):
-                raise RuntimeError(f"attention: {name}: head vectors must be contiguous, 16-byte aligned, strides multiples of 8, a token's below 2^24")
-            op.ptrs.append(t.data_ptr())
-            op.strides += st
+        op.sizes, op.tensors = (B, H, k.shape[2], Lq, k.shape[1], D), (q, k, v)
+        op.ptrs, op.strides = [a[0] for a in at], at[0][1] + at[1][1] + at[2][1]
+        return op
+
+    @classmethod
+    def fresh(cls, sizes, like):
+        """New tensors of these sizes, nothing written."""
+        B, H, Hkv, Lq, Lk, D = sizes
+        op = cls()
+        op.sizes, op.tensors = sizes, tuple(like.new_empty(s) for s in ((B, Lq, H, D), (B, Lk, Hkv, D), (B, Lk, Hkv, D)))
+        op.ptrs, op.strides = [t.data_ptr() for t in op.tensors], [Lq * H * D, H * D, D] + [Lk * Hkv * D, Hkv * D, D] * 2
         return op
 
     @classmethod
@@ -1683,14 +1695,14 @@ class AttnOperands:
         D = W // (heads + 2 * kv_heads)
         if D not in HEAD_SIZES:
             raise RuntimeError(f"attention: head size {D} is not one of {HEAD_SIZES}")
-        op = cls()
-        sb, sl = cls._axis(qkv, 2)
-        if not cls.readable(qkv, (sb, sl)):
+        at = cls.place(qkv)
+        if at is None:
             raise RuntimeError("attention: qkv: a token's channels must be contiguous, 16-byte aligned, strides multiples of 8, a token's below 2^24")
-        p = qkv.data_ptr()
+        p, st = at
+        op = cls()
         op.sizes, op.tensors = (B, heads, kv_heads, N, N, D), (qkv,)
         op.ptrs = [p, p + 2 * heads * D, p + 2 * (heads + kv_heads) * D] if p else [0, 0, 0]
-        op.strides = [sb, sl, D] * 3
+        op.strides = (st + [D]) * 3
         return op
 
 
