@@ -14,6 +14,10 @@
 // product as they stand (its K order follows the accumulator's: 4 keys of one half, 4 of the other), while the A operand comes
 // out of LDS through the transposing read.  Probabilities and score gradients are rounded to bf16 only as operands of these
 // products; maxima, sums, statistics and the table's gradient stay in fp32.
+//
+// Times below: us on one MI355X, where a 2 GB copy reaches 5.05 TB/s and an 8192^3 bf16 product of the library 1130 TFLOP/s.  "32 px":
+// 32 samples of a 32x32 map, 4 heads of 64; "64 px": 8 of 64x64, 2 heads of 64, capped scores; "128 px": 4 of 128x128, one head of 64;
+// "line": 2 of 4096 tokens, 4 query heads on 2 of 128.
 #include <type_traits>
 
 #include "common.h"
@@ -21,10 +25,9 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
-// rows of a streamed tile (keys forward and in dq, queries in dk / dv): two buffers of two operands are 32 KB of LDS either way
+// rows of a streamed tile (keys forward and in dq, queries in dk / dv): two buffers of two operands are 32 KB of LDS at head sizes 64 and
+// 128, 16 KB at 32
 constexpr int kt_of(int D) { return D == 128 ? 32 : 64; }
-// ... of dq, which has the table's gradient in LDS too: 16 or 32 KB, three workgroups a compute unit at head sizes up to 64
-constexpr int kt_dq(int D) { return D == 128 ? 32 : 64; }
 constexpr int BLK = 128;                  // rows a workgroup owns: 4 waves x 32
 constexpr int WIN_PAD = 4;
 // LDS bytes for the window: with the tiles (32 KB) three workgroups a compute unit forward, two of dq with its blocks (69 KB)
@@ -327,11 +330,18 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 }
 
 // ======================================================================================================= forward
+// A workgroup owns 128 queries of a head, a wave 32 of them, and streams tiles of keys and values (64 rows, 32 at head size 128) through
+// two LDS buffers: the next tile's loads run under the whole of this one's work.  What bounds it is issue, not a pipe: of the cycles of a
+// SIMD at 128 px the matrix instructions take 34 %, the vector ones (16 exponentials of 4 slots each, 60 others a 32 x 32 block) 54 %, and
+// with two or three waves they overlap little.  Leaving out, one at a time, the exponentials, half of the second product, the bias reads
+// or the tiles' loads shortens it by 9 .. 12 % each; both blocks' first products ahead of the softmax change nothing.  Three workgroups
+// a compute unit at head size 64 (registers and LDS; four spill), two at 128.  32 px 50 without bias, 63 with; 128 px 360 .. 400 (690 ..
+// 760 TFLOP/s; its 512 workgroups are two a compute unit), three times its samples 850 TFLOP/s.
 // LDS: K[2] V[2] tiles | window | table of the segment's places (BIAS 1).
 // FINE: the probabilities go into the second product as three bf16 terms (24 bits): delta = do . o must be that exact where the fp32
 // gradient of the table is wanted, whose sums cancel.  Its error against 64 bits over forms of 18 to 8192 tokens: one term 5e-4, two
-// 0.6 .. 4e-6, three 0.2 .. 0.7e-6, as fp32 arithmetic leaves.  V's operands serve all three.  32 samples of 32x32, 4 heads of 64: one
-// term 48 us, two 74, three 88 (the terms' subtractions, not the products).
+// 0.6 .. 4e-6, three 0.2 .. 0.7e-6, as fp32 arithmetic leaves.  V's operands serve all three.  32 px: one term 63, two 74, three 84 .. 88
+// (the terms' subtractions, not the products).
 template <int D, int BIAS, bool CAP, bool FINE>
 __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -513,7 +523,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
 // At most 32 (query, head) pairs share a key / value head: all of them are the lanes of ONE product, so keys and values are read once
 // however many heads share them, and the keys are cut into `splits` runs for as many workgroups.  Bound by reading keys and values: a
 // wave streams blocks of 32 keys of its own (two buffers, no barrier in the loop), and the waves', then the runs', (maximum, sum,
-// output) are joined in a fixed order.  part: (B, Hkv, splits, 32, D + 2) fp32: output, maximum, sum.
+// output) are joined in a fixed order.  part: (B, Hkv, splits, 32, D + 2) fp32: output, maximum, sum; one run writes the rows itself.
+// One query, 4 samples of 16384 keys, 8 heads on 2 of 128 (67 MB): 20 + 4, 3.3 TB/s; 256 samples of 1024 keys, 8 heads of 64 (537 MB):
+// 114, 4.7 TB/s.
 // LDS: for each wave K[2] V[2] of 32 rows; the joining reuses it.
 template <int D> struct WaveDma {
     static constexpr int NP = D / 16;                                // 1 KB pieces of a block
@@ -733,22 +745,25 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
 //   BLOCKS    where 32 aligned tokens lie in one row of the grid (columns a multiple of 32, or a single row): within a 32 x 32 block
 //             the offset is one number plus (query - key), 63 sums.  A wave puts its block into LDS of its own (no barrier), rows
 //             of 32 values and 40 zeros: a lane then adds up one diagonal, 32 reads at fixed distances that run off the block into
-//             zeros, no comparison.  part (b, h, query group, key group, 64).  (Adding with ds_add_f32 instead took 2.8 times the
-//             whole kernel's time: 728 us against 264 with diagonals at 32 samples x 4 heads x 1024 tokens.)
+//             zeros, no comparison.  part (b, h, query group, key group, 64).  Adding with ds_add_f32 instead: 728, 32 px.  The sums
+//             of a tile are stored one tile later: the wait for the next tile's loads would wait for a store that has just gone out.
 //   DIAGONALS any other grid: a pair is known by its distance i - j and by whether the column of i wraps (class 0: dx >= 0, class 1:
 //             dx < 0).  ds goes through LDS and a thread adds up one diagonal of the tile; a diagonal stays with its thread (distance
-//             mod 256) over the tiles it crosses and is stored once: part (b, h, query block, class, distance).
+//             mod 256) over the tiles it crosses and is stored once: part (b, h, query block, class, distance).  Taken where BLOCKS
+//             would do it costs more: 32 px 224 + 18 against 128 + 26, same run.
+// Three products a block where the forward pass has two.  32 px: 68 without bias, 79 with, 107 .. 128 with the table's sums (16 writes and
+// 32 reads of 4 bytes more a lane and block), 64 px 250, line 172.  Two workgroups a compute unit (three at head size 32).
 // LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
 enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
 constexpr int BS = 72;                    // floats from row to row of a block: rows 4 apart (a wave's halves) are 32 banks apart
 constexpr int block_rows(int D) { return D == 128 ? 16 : 32; }       // (16: a block goes through in two halves, for two workgroups' LDS)
 constexpr int block_floats(int D) { return 32 + block_rows(D) * BS; }
-constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * block_floats(D) * 4 : dt == DT_DIAGONALS ? kt_dq(D) * BLK * 4 : 0; }
+constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * block_floats(D) * 4 : dt == DT_DIAGONALS ? kt_of(D) * BLK * 4 : 0; }
 
 template <int D, int BIAS, bool CAP, int DT>
 __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    constexpr int BR = block_rows(D), KT = kt_dq(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
+    constexpr int BR = block_rows(D), KT = kt_of(D), TB = KT * 2 * D, KS = D / 16, DB = D / 32;
     float* dsl = reinterpret_cast<float*>(smem + 4 * TB);
     char* win = smem + 4 * TB + dt_lds(DT, D);
     int* at = reinterpret_cast<int*>(win + a.win_bytes);
@@ -805,8 +820,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
     float* part = DT == DT_DIAGONALS ? a.part + (int64_t)id * 2 * a.span
                                      : DT == DT_BLOCKS ? a.part + ((int64_t)id * 4 + wave) * n_kg * 64 : nullptr;
     const int d_min = tq0 - (nt * KT - 1);
-    float hold[KT / 32];                                             // BLOCKS: a tile's sums, stored a tile later: the wait for the next tile's
-                                                                     // loads would wait for a store that has just gone out
+    float hold[KT / 32];                                             // BLOCKS: a tile's sums until they are stored
 
     Dma<D, KT> sk, sv;
     Places<BIAS> pl;
@@ -952,7 +966,8 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
 
 // ---- the table's gradient from the partials: sums over samples and places first, then by bucket.
 // BLOCKS.  by_block (H, classes, 64): a class is (row difference, column-group difference) of a block's query and key groups, G =
-// columns / 32 groups a row (a single row: G = all of them).  grid (classes, H), 16 row lanes x 64 places; `more`: samples behind those that are summed already.
+// columns / 32 groups a row (a single row: G = all of them).  grid (classes, H), 16 row lanes x 64 places; `more`: samples behind those
+// that are summed already.
 __global__ __launch_bounds__(1024) void attn_block_sums_kernel(AttnArgs a, float* by_block, bool more, int q_rows, int k_rows, int gq, int gk) {
     __shared__ float red[1024];
     const int cls = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, r = threadIdx.x >> 6;
@@ -1060,6 +1075,9 @@ __global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const
 // A workgroup owns 128 keys of one key / value head and streams the queries of every head that shares it: scores here are
 // queries x keys, a lane holds one key.  No sum leaves the workgroup; where keys and heads alone are too few workgroups for the chip,
 // the tiles of queries are cut into `splits` runs whose fp32 sums a second launch adds up: part (splits, B, Hkv, Lk, 2 D).
+// Four products a block; the row sums' logarithm and delta come in as the products' initial values, which saves their subtraction.
+// 32 px 82 without bias, 95 .. 107 with, 64 px 239, line 231 + 9.  Two waves a SIMD at head size 64 (three spill), one at 128: dk, dv
+// and the wave's own keys and values are 384 registers there, and with two waves they spill.
 // LDS: Q[2] dO[2] | lse[2][64] | delta[2][64] | window | table of the segment's places (BIAS 1).
 template <int D, int BIAS, bool CAP>
 __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {
@@ -1416,7 +1434,7 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     const int ks = kv_splits(d);
     z.kv = ks > 1 ? (int64_t)ks * d->B * d->Hkv * d->Lk * 2 * d->D : 0;
     if (!dt || d->Lq == 0 || d->Lk == 0) return z;
-    const int KT = kt_dq(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
+    const int KT = kt_of(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
         z.mode = DT_BLOCKS;
         z.part = (int64_t)d->H * n_qb * 4 * n_kt * (KT / 32) * 64;
@@ -1527,8 +1545,6 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
 
     if (d->Lq > 0) {
         const int bias = bias_mode(d, 0);
-        a.kt = kt_dq(d->D);
-        a.n_kt = ceil_div(d->Lk, a.kt);
         const Window w = window_of(bias, d->Lq, d->Lk, a.rows, a.cols, a.kt, z.mode ? WIN_DQ : WIN_FWD);
         RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
         a.seg_tiles = w.tiles;
@@ -1563,7 +1579,6 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
     }
     if (d->Lk > 0) {
         const int bias = d->Lq > 0 ? bias_mode(d, d->q_start) : 0;
-        a.kt = kt_of(d->D);
         const Window w = window_of(bias, d->Lk, d->Lq, a.rows, a.cols, a.kt, WIN_FWD);
         RGBD_REQUIRE(bias == 0 || w.tiles > 0, "%s: the bias of one tile does not fit (%d x %d grid)", who, a.rows, a.cols);
         a.seg_tiles = w.tiles;
