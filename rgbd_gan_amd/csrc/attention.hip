@@ -1077,7 +1077,7 @@ __global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const
 // the tiles of queries are cut into `splits` runs whose fp32 sums a second launch adds up: part (splits, B, Hkv, Lk, 2 D).
 // Four products a block; the row sums' logarithm and delta come in as the products' initial values, which saves their subtraction.
 // 32 px 82 without bias, 95 .. 107 with, 64 px 239, line 231 + 9.  Two waves a SIMD at head size 64 (three spill), one at 128: dk, dv
-// and the wave's own keys and values are 384 registers there, and with two waves they spill.
+// and the wave's own keys and values are 192 registers there, a block's scores and operands the rest of 450; within 256 they spill.
 // LDS: Q[2] dO[2] | lse[2][64] | delta[2][64] | window | table of the segment's places (BIAS 1).
 template <int D, int BIAS, bool CAP>
 __global__ __launch_bounds__(256, D == 128 ? 1 : D == 64 ? 2 : 3) void attn_dkv_kernel(AttnArgs a) {

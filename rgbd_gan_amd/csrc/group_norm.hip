@@ -14,8 +14,8 @@
 //             the map fits there.
 // Measured (us on one MI355X; a 67 MB copy, which the last-level cache holds, runs at 7.2 TB/s, a 2 GB one at 5.05): resident, 32 x 32x32 x
 // 256 bf16 in 32 groups: 16 forward (34 MB at 2.1 TB/s: one workgroup of 1024 threads a compute unit reads, reduces and writes in turn,
-// nothing runs under the barriers), 20 + 4 backward; slabs, 32 x 128x128 x 64 in 16 groups with SiLU: 20 + 26 forward, 32 + 36 backward, 5.0 TB/s over
-// the 570 MB that the two passes move in all (270 if every map were read once, which needs a sample's workgroups to wait for each other).
+// nothing runs under the barriers), 20 + 4 backward; slabs, 32 x 128x128 x 64 in 16 groups with SiLU: 20 + 26 forward, 32 + 36 backward, 4.8 TB/s over
+// the 537 MB that the four launches move (335 if each pass read its maps once, which needs a sample's workgroups to wait for each other).
 // 16 and 8 vectors a thread instead of 8 and 4 spill; four workgroups a compute unit for the slabs' sums.
 // Statistics never come from sums of squares: a thread's eight pixels give a mean and a sum of squared deviations, and these
 // pairs are merged (Chan, Golub, LeVeque 1979), so a mean far from zero costs no digits.  Everything is summed in fp32 in an
