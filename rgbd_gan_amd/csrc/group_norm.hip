@@ -13,8 +13,8 @@
 //             partials of its sample (a few KB) and writes the result; the second read comes out of the last-level cache while
 //             the map fits there.
 // Measured (us on one MI355X; a 67 MB copy, which the last-level cache holds, runs at 7.2 TB/s, a 2 GB one at 5.05): resident, 32 x 32x32 x
-// 256 bf16 in 32 groups: 16 forward (34 MB at 2.1 TB/s: one workgroup of 1024 threads a compute unit reads, reduces and writes in turn,
-// nothing runs under the barriers), 20 + 4 backward; slabs, 32 x 128x128 x 64 in 16 groups with SiLU: 20 + 26 forward, 32 + 36 backward, 4.8 TB/s over
+// 256 bf16 in 32 groups: 14 forward (34 MB at 2.4 TB/s: one workgroup of 1024 threads a compute unit reads, reduces and writes in turn,
+// nothing runs under the barriers), 15 + 4 backward; slabs, 32 x 128x128 x 64 in 16 groups with SiLU: 20 + 26 forward, 32 + 36 backward, 4.8 TB/s over
 // the 537 MB that the four launches move (335 if each pass read its maps once, which needs a sample's workgroups to wait for each other).
 // 16 and 8 vectors a thread instead of 8 and 4 spill; four workgroups a compute unit for the slabs' sums.
 // Statistics never come from sums of squares: a thread's eight pixels give a mean and a sum of squared deviations, and these
@@ -164,6 +164,13 @@ __device__ __forceinline__ void sum_over_group(const float* ch, float* out, int 
 }
 
 // ---- resident form ------------------------------------------------------------------------------------------------------
+// Workgroups go round the 8 XCDs: each XCD gets the channel runs of the same samples, whose lines (two runs each) its L2 then reads once
+// (32 x 32x32 x 256: forward 16.4 -> 15.2 us, backward 20.4 -> 15.7).
+__device__ __forceinline__ int sample_run() {
+    const int id = blockIdx.y * gridDim.x + blockIdx.x, total = gridDim.x * gridDim.y, q = total >> 3, r = total & 7, x = id & 7;
+    return x * q + min(x, r) + (id >> 3);
+}
+
 template <typename T, int V, int E, int ACT>
 __global__ __launch_bounds__(1024) void gn_fwd_resident(GnArgs a) {
     extern __shared__ float lds[];                        // red (pl * cw) | per group: mean, rstd
@@ -171,7 +178,7 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(GnArgs a) {
     float* gm = lds + a.pl * a.cw;
     float* gr = gm + a.cw / a.cpg;
     const int groups = a.cw / a.cpg;
-    const int b = blockIdx.y, c0 = blockIdx.x * a.cw;
+    const int id = sample_run(), b = id / gridDim.x, c0 = id % gridDim.x * a.cw;
     const int p = threadIdx.x / a.nc, j = threadIdx.x - p * a.nc;
     const bool live = p < a.pl;
     const T* x = reinterpret_cast<const T*>(a.x) + (int64_t)b * a.N * a.C + c0 + j * V;
@@ -209,15 +216,18 @@ __global__ __launch_bounds__(1024) void gn_fwd_resident(GnArgs a) {
             for (int i = 0; i < V; ++i) { const float d = xs[e].get(i) - mean[i]; acc[i] += d * d; }
     sum_over_pixels<V>(red, acc, p, j, a.pl, a.cw, live);
     sum_over_group(red, gr, groups, a.cpg);
-    if ((int)threadIdx.x < groups) {
-        const int64_t o = (int64_t)b * a.G + c0 / a.cpg + threadIdx.x;
-        a.mean[o] = gm[threadIdx.x] * inv;
-        a.rstd[o] = 1.f / sqrtf(gr[threadIdx.x] * inv + a.eps);
+    for (int g = threadIdx.x; g < groups; g += blockDim.x) {
+        const int64_t o = (int64_t)b * a.G + c0 / a.cpg + g;
+        const float r = 1.f / sqrtf(gr[g] * inv + a.eps);
+        a.mean[o] = gm[g] * inv;
+        a.rstd[o] = r;
+        gr[g] = r;
     }
+    __syncthreads();
     if (!live) return;
     float scale[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) scale[i] = 1.f / sqrtf(gr[gi[i]] * inv + a.eps);
+    for (int i = 0; i < V; ++i) scale[i] = gr[gi[i]];
     T* y = reinterpret_cast<T*>(a.out) + (int64_t)b * a.N * a.C + c0 + j * V;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -238,7 +248,7 @@ __global__ __launch_bounds__(1024) void gn_bwd_resident(GnArgs a) {
     const int groups = a.cw / a.cpg;
     float* s1 = lds + a.pl * a.cw;
     float* s2 = s1 + groups;
-    const int b = blockIdx.y, c0 = blockIdx.x * a.cw;
+    const int id = sample_run(), b = id / gridDim.x, c0 = id % gridDim.x * a.cw;
     const int p = threadIdx.x / a.nc, j = threadIdx.x - p * a.nc;
     const bool live = p < a.pl;
     const int64_t base = (int64_t)b * a.N * a.C + c0 + j * V;
