@@ -1671,6 +1671,15 @@ def fold_weight(W, mode, Cop, Cip):
 
 
 # ---- group norm and attention over feature maps
+def _once(backward):
+    """once_differentiable, whose wrapping of the results is left out (4 us of the host's time) where no graph of them is wanted."""
+    marked = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return marked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, groups, eps, act, slope):
@@ -1680,7 +1689,7 @@ class _GroupNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, gamma, beta, stats = ctx.saved_tensors
         return *kernels.group_norm_bwd(x, dy.contiguous(), gamma, beta, stats, *ctx.spec), None, None, None, None
@@ -1747,7 +1756,7 @@ class _Attention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_o):
         q, k, v, table, lengths, *kept = ctx.saved_tensors
         op = kernels.AttnOperands.of(q, k, v)
@@ -1769,7 +1778,7 @@ class _AttentionPacked(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, d_o):
         qkv, table, lengths, *kept = ctx.saved_tensors
         dqkv = qkv.new_empty(qkv.shape)

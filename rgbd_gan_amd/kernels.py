@@ -1554,50 +1554,52 @@ def _launch_stream(what, *tensors):
     return _raw_stream_of(cur)
 
 
-def _gn_sizes(x, gamma, beta, groups, act):
-    if not torch.is_tensor(x) or x.dim() < 2:
-        raise RuntimeError("group_norm: x must have a batch and a channel axis, (B, ..., C)")
-    dt = x.dtype
-    if dt != BF16 and dt != F32:
-        raise RuntimeError(f"group_norm: x must be bf16 or fp32, got {dt}")
+@functools.lru_cache(maxsize=1024)
+def _gn_plan(shape, dtype, groups, act):
+    """Checked sizes of a map and what the library asks for them: B, N, C, element code, workspace floats forward and backward."""
+    if dtype != BF16 and dtype != F32:
+        raise RuntimeError(f"group_norm: x must be bf16 or fp32, got {dtype}")
     if act not in ACTS:
         raise RuntimeError(f"group_norm: act must be one of {sorted(k for k in ACTS if k)}, got {act!r}")
-    shape = x.shape
     B, C = shape[0], shape[-1]
-    groups = int(groups)
     if groups < 1 or C < 1 or C % groups:
         raise RuntimeError(f"group_norm: {groups} groups do not divide {C} channels")
-    if gamma.shape != (C,):
-        raise RuntimeError(f"group_norm: gamma must have shape ({C},), got {tuple(gamma.shape)}")
-    if beta.shape != (C,):
-        raise RuntimeError(f"group_norm: beta must have shape ({C},), got {tuple(beta.shape)}")
     N = 1
     for n in shape[1:-1]:
         N *= n
-    _chk(x, dt, "x"); _chk(gamma, F32, "gamma"); _chk(beta, F32, "beta")
-    return B, N, C, groups, 0 if dt == BF16 else 1
+    dt, ws = 0 if dtype == BF16 else 1, []
+    for backward in (0, 1):
+        ws.append(_lib.load().rgbd_group_norm_workspace(B, N, C, groups, dt, backward))
+        if ws[-1] < 0:
+            _lib.check(-1, "rgbd_group_norm_workspace")
+    return B, N, C, dt, *ws
 
 
-@functools.lru_cache(maxsize=256)
-def _gn_workspace_floats(B, N, C, groups, dtype, backward):
-    n = _lib.load().rgbd_group_norm_workspace(B, N, C, groups, dtype, backward)
-    if n < 0:
-        _lib.check(-1, "rgbd_group_norm_workspace")
-    return n
+def _gn_sizes(x, gamma, beta, groups, act):
+    if not torch.is_tensor(x) or x.dim() < 2:
+        raise RuntimeError("group_norm: x must have a batch and a channel axis, (B, ..., C)")
+    plan = _gn_plan(x.shape, x.dtype, groups, act)
+    C = (plan[2],)
+    if gamma.shape != C:
+        raise RuntimeError(f"group_norm: gamma must have shape {C}, got {tuple(gamma.shape)}")
+    if beta.shape != C:
+        raise RuntimeError(f"group_norm: beta must have shape {C}, got {tuple(beta.shape)}")
+    _chk(x, x.dtype, "x"); _chk(gamma, F32, "gamma"); _chk(beta, F32, "beta")
+    return plan
 
 
 def group_norm_fwd(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
     """x (B, ..., C) bf16 or fp32, gamma, beta (C,) fp32 -> y like x, stats (2, B, groups) fp32: the groups' means and 1 / sqrt(var + eps)."""
-    B, N, C, groups, dt = _gn_sizes(x, gamma, beta, groups, act)
+    groups = int(groups)
+    B, N, C, dt, n, _ = _gn_sizes(x, gamma, beta, groups, act)
     if not eps >= 0:
         raise RuntimeError(f"group_norm: eps must not be negative, got {eps}")
     stream = _launch_stream("group_norm", x, gamma, beta)
     y = torch.empty_like(x)
-    n = _gn_workspace_floats(B, N, C, groups, dt, 0)
     # statistics and workspace in one allocation
-    buf = torch.empty(2 * B * groups + n, dtype=F32, device=x.device)
+    buf = gamma.new_empty(2 * B * groups + n)
     p = buf.data_ptr()
-    rc = _timed("gn_fwd", 0, 2 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_fwd(
+    rc = _timed("gn_fwd", 0, (4 + 4 * dt) * B * N * C, lambda: _lib.load().rgbd_group_norm_fwd(
         x.data_ptr(), gamma.data_ptr(), beta.data_ptr(), y.data_ptr(), p, p + 4 * B * groups, p + 8 * B * groups, B, N, C, groups, dt,
         ACTS[act], eps, slope, stream))
     if rc:
@@ -1607,15 +1609,16 @@ def group_norm_fwd(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
 
 def group_norm_bwd(x, dy, gamma, beta, stats, groups, act=None, slope=0.2):
     """-> dx like x, dgamma, dbeta (C,) fp32."""
-    B, N, C, groups, dt = _gn_sizes(x, gamma, beta, groups, act)
+    groups = int(groups)
+    B, N, C, dt, _, n = _gn_sizes(x, gamma, beta, groups, act)
     _chk(dy, x.dtype, "dy"); _chk(stats, F32, "stats")
     if dy.shape != x.shape or stats.numel() != 2 * B * groups:
         raise RuntimeError("group_norm: dy or the statistics do not match x")
     stream = _launch_stream("group_norm", x, gamma, beta, dy, stats)
     dx, dgamma, dbeta = torch.empty_like(x), torch.empty_like(gamma), torch.empty_like(beta)
-    ws = torch.empty(_gn_workspace_floats(B, N, C, groups, dt, 1), dtype=F32, device=x.device)
+    ws = gamma.new_empty(n)
     p = stats.data_ptr()
-    rc = _timed("gn_bwd", 0, 3 * x.numel() * x.element_size(), lambda: _lib.load().rgbd_group_norm_bwd(
+    rc = _timed("gn_bwd", 0, (6 + 6 * dt) * B * N * C, lambda: _lib.load().rgbd_group_norm_bwd(
         x.data_ptr(), dy.data_ptr(), gamma.data_ptr(), beta.data_ptr(), p, p + 4 * B * groups, dx.data_ptr(), dgamma.data_ptr(),
         dbeta.data_ptr(), ws.data_ptr(), B, N, C, groups, dt, ACTS[act], slope, stream))
     if rc:
@@ -1763,14 +1766,14 @@ def attention_fwd(op, table=None, buckets=None, lengths=None, scale=None, cap=0.
     lse (B, H, Lq) fp32 (else None).  fine: what the table's gradient needs of o (probabilities with 24 bits in the second product)."""
     B, H, Hkv, Lq, Lk, D = op.sizes
     t = op.tensors[0]
-    o = torch.empty((B, Lq, H, D), dtype=BF16, device=t.device)
+    o = t.new_empty((B, Lq, H, D))
     o_lo = torch.empty_like(o) if keep else None
     lse = torch.empty((B, H, Lq), dtype=F32, device=t.device) if keep else None
     d, stream = _attn_desc(op, table, buckets, lengths, D ** -0.5 if scale is None else float(scale), cap, q_start,
                            lse.data_ptr() if keep else 0, int(fine))
     lib = _lib.load()
     n = _attn_workspace(op, buckets, q_start, 0, lambda: lib.rgbd_attention_fwd_workspace(ctypes.byref(d)))
-    ws = torch.empty(n, dtype=F32, device=t.device) if n else None
+    ws = lse.new_empty(n) if n and keep else torch.empty(n, dtype=F32, device=t.device) if n else None
     rc = _timed("attn_fwd", 4 * B * H * Lq * Lk * D, 4 * B * D * (H * Lq + Hkv * Lk), lambda: lib.rgbd_attention_fwd(
         ctypes.byref(d), o.data_ptr(), o_lo.data_ptr() if keep else 0, ws.data_ptr() if n else 0, stream))
     if rc:
@@ -1796,7 +1799,7 @@ def attention_bwd(op, out, d_o, o, o_lo, lse, table=None, buckets=None, lengths=
         (dtable.data_ptr(), buckets.order.data_ptr(), buckets.start.data_ptr()) if want_table else (0, 0, 0)))
     lib = _lib.load()
     n = _attn_workspace(op, buckets, q_start, 1 + want_table, lambda: lib.rgbd_attention_bwd_workspace(ctypes.byref(d), int(want_table)))
-    ws = torch.empty(n, dtype=F32, device=d_o.device)
+    ws = lse.new_empty(n)
     rc = _timed("attn_bwd", 10 * B * H * Lq * Lk * D, 8 * B * D * (H * Lq + Hkv * Lk), lambda: lib.rgbd_attention_bwd(
         ctypes.byref(d), ctypes.byref(g), ws.data_ptr(), stream))
     if rc:
