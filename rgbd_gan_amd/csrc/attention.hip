@@ -45,6 +45,7 @@ struct AttnArgs {
     int B, H, Hkv, rep, Lq, Lk;
     int rows, cols, pos_cols, q_start, n_buckets;
     int kt, n_qb, n_kb, n_kt, seg_tiles, win_bytes, splits;
+    float* runs; int64_t run_floats;      // dq in runs of keys: their fp32 sums (splits, B, Lq, H, D)
     int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
     float scale, cap;
 };
@@ -752,13 +753,17 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
 //             mod 256) over the tiles it crosses and is stored once: part (b, h, query block, class, distance).  Taken where BLOCKS
 //             would do it costs more: 32 px 224 + 18 against 128 + 26, same run.
 // Three products a block where the forward pass has two.  32 px: 68 without bias, 79 with, 107 .. 128 with the table's sums (16 writes and
-// 32 reads of 4 bytes more a lane and block), 64 px 250, line 172.  Two workgroups a compute unit (three at head size 32).
-// LDS: K[2] V[2] | at[2][64] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
+// 32 reads of 4 bytes more a lane and block), 64 px 250, line 143 + 9.  Two workgroups a compute unit (three at head size 32).
+// Few workgroups: the keys are cut into `splits` runs whose fp32 dq a second launch adds up (a run has its own diagonals, and its own blocks).
+// LDS: K[2] V[2] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
 enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
 constexpr int BS = 72;                    // floats from row to row of a block: rows 4 apart (a wave's halves) are 32 banks apart
 constexpr int block_rows(int D) { return D == 128 ? 16 : 32; }       // (16: a block goes through in two halves, for two workgroups' LDS)
 constexpr int block_floats(int D) { return 32 + block_rows(D) * BS; }
 constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * block_floats(D) * 4 : dt == DT_DIAGONALS ? kt_of(D) * BLK * 4 : 0; }
+
+// First of n tiles of a run.
+__device__ __forceinline__ int run_first(int n, int runs, int run) { return min(n, (n + runs - 1) / runs * run); }
 
 template <int D, int BIAS, bool CAP, int DT>
 __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
@@ -770,7 +775,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
     const int n_kg = a.n_kt * (KT / 32);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
-    const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
+    const int split = id % a.splits, own = id / a.splits, qb = own % a.n_qb, bh = own / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row = qb * BLK + wave * 32 + (lane & 31);
     const bool live = row < a.Lq;
@@ -800,14 +805,14 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
         }
     }
     delta = other_half_sum(delta);
-    if (live && half == 0) a.delta[(int64_t)bh * a.Lq + row] = delta;
+    if (live && half == 0 && split == 0) a.delta[(int64_t)bh * a.Lq + row] = delta;
     if (!live) delta = 0.f;
     const float lse = live ? a.lse[(int64_t)bh * a.Lq + row] : NO_ROW;
 
     const int len = keys_of(a, b);
-    const int nt = (len + KT - 1) / KT;
-    const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
-    const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
+    const int nt = (len + KT - 1) / KT, t0 = run_first(nt, a.splits, split), t1 = run_first(nt, a.splits, split + 1);
+    const unsigned short* kp = a.k + b * a.k_sb + (int64_t)t0 * KT * a.k_sl + hk * a.k_sh;
+    const unsigned short* vp = a.v + b * a.v_sb + (int64_t)t0 * KT * a.v_sl + hk * a.v_sh;
     const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
     const int pq0 = BIAS ? pos_of(tq0, a.pos_cols) : 0, pq1 = BIAS ? pos_of(tq1, a.pos_cols) : 0;
     const int lane_off = BIAS ? 4 * (pq1 - pos_of(min(a.q_start + row, tq1), a.pos_cols)) + Places<BIAS>::half_off(a, half) : 0;
@@ -818,17 +823,17 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
     float sum0 = 0.f, sum1 = 0.f;                                    // the thread's diagonal, by class
     // DIAGONALS: partials of this workgroup, place 0 = the smallest distance it meets
     float* part = DT == DT_DIAGONALS ? a.part + (int64_t)id * 2 * a.span
-                                     : DT == DT_BLOCKS ? a.part + ((int64_t)id * 4 + wave) * n_kg * 64 : nullptr;
+                                     : DT == DT_BLOCKS ? a.part + ((int64_t)own * 4 + wave) * n_kg * 64 : nullptr;
     const int d_min = tq0 - (nt * KT - 1);
     float hold[KT / 32];                                             // BLOCKS: a tile's sums until they are stored
 
     Dma<D, KT> sk, sv;
     Places<BIAS> pl;
-    int seg_t = 0;
-    if (BIAS) pl.init(a, 0);
-    if (nt > 0) {
-        sk.init(kp, a.k_sl, len, smem);
-        sv.init(vp, a.v_sl, len, smem + 2 * TB);
+    int seg_t = t0;
+    if (BIAS) pl.init(a, t0 * KT);
+    if (t0 < t1) {
+        sk.init(kp, a.k_sl, len - t0 * KT, smem);
+        sv.init(vp, a.v_sl, len - t0 * KT, smem + 2 * TB);
         sk.next(a.k_sl, 0);
         sv.next(a.v_sl, 0);
         dma_wait();
@@ -839,7 +844,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
         constexpr int P = decltype(parity)::value;
         const char* kc = smem + P * TB;
         const char* vc = smem + (2 + P) * TB;
-        if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
+        if (BIAS && (t == t0 || t == seg_t + a.seg_tiles)) {
             __syncthreads();
             seg_t = t;
             pl.blk = 0;
@@ -848,10 +853,10 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             Places<BIAS>::table(at, a, t * KT, n, a.Lk - 1);
         }
         __syncthreads();
-        if (DT == DT_BLOCKS && t > 0)
+        if (DT == DT_BLOCKS && t > t0)
 #pragma unroll
             for (int u = 0; u < KT / 32; ++u) part[(KT / 32 * (t - 1) + u) * 64 + lane] = hold[u];
-        if (t + 1 < nt) {
+        if (t + 1 < t1) {
             sk.next(a.k_sl, (P ^ 1) * TB);
             sv.next(a.v_sl, (P ^ 1) * TB);
         }
@@ -937,7 +942,7 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
                         x -= x == r ? a.cols : 0;                    // the key's own row ends
                     }
                 }
-                if (c + KT >= BLK || t + 1 == nt) {                        // the diagonal leaves the workgroup's rows
+                if (c + KT >= BLK || t + 1 == t1) {                        // the diagonal leaves the workgroup's rows, or the run ends
                     part[dist - d_min] = sum0;
                     part[a.span + dist - d_min] = sum1;
                     sum0 = sum1 = 0.f;
@@ -945,14 +950,23 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
             }
         }
     };
-    for (int t = 0; t < nt; t += 2) {
+    for (int t = t0; t < t1; t += 2) {
         tile(t, std::integral_constant<int, 0>{});
-        if (t + 1 < nt) tile(t + 1, std::integral_constant<int, 1>{});
+        if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
     }
-    if (DT == DT_BLOCKS && nt > 0)
+    if (DT == DT_BLOCKS && t0 < t1)
 #pragma unroll
-        for (int u = 0; u < KT / 32; ++u) part[(KT / 32 * (nt - 1) + u) * 64 + lane] = hold[u];
+        for (int u = 0; u < KT / 32; ++u) part[(KT / 32 * (t1 - 1) + u) * 64 + lane] = hold[u];
     if (!live) return;
+    if (a.splits > 1) {
+        float* p = a.runs + split * a.run_floats + (((int64_t)b * a.Lq + row) * a.H + h) * D + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(p + 32 * d + 8 * g) = f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        return;
+    }
     unsigned short* qo = a.dq + b * a.dq_sb + (int64_t)row * a.dq_sl + h * a.dq_sh + 4 * half;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -962,6 +976,21 @@ __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs 
                              pack_bf16x2(acc[d][4 * g + 2] * a.scale, acc[d][4 * g + 3] * a.scale)};
             *reinterpret_cast<u32x2*>(qo + 32 * d + 8 * g) = w;
         }
+}
+
+// dq from the runs' sums: four values a thread, grid (sample, query, head, D / 4) / 256.
+__global__ __launch_bounds__(256) void attn_dq_sum_kernel(AttnArgs a, int D) {
+    const int64_t e = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
+    if (e >= a.run_floats) return;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < a.splits; ++i) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.runs + i * a.run_floats + e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += v[k];
+    }
+    const int64_t row = e / D / a.H, b = row / a.Lq;
+    unsigned short* o = a.dq + b * a.dq_sb + (row - b * a.Lq) * a.dq_sl + e / D % a.H * a.dq_sh + e % D;
+    *reinterpret_cast<u32x2*>(o) = u32x2{pack_bf16x2(s[0] * a.scale, s[1] * a.scale), pack_bf16x2(s[2] * a.scale, s[3] * a.scale)};
 }
 
 // ---- the table's gradient from the partials: sums over samples and places first, then by bucket.
@@ -1038,12 +1067,12 @@ __global__ __launch_bounds__(1024) void attn_dist_kernel(AttnArgs a, float* by_d
     const int i = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
     const int cls = blockIdx.y & 1, h = blockIdx.y >> 1, dist = i + d0;
     float s = 0.f;
-    for (int e = r; e < a.B * a.n_qb; e += 16) {
-        const int qb = e % a.n_qb, b = e / a.n_qb;
-        const int nt = (keys_of(a, b) + a.kt - 1) / a.kt;
+    for (int e = r; e < a.B * a.n_qb * a.splits; e += 16) {
+        const int split = e % a.splits, qb = e / a.splits % a.n_qb, b = e / a.splits / a.n_qb;
+        const int nt = (keys_of(a, b) + a.kt - 1) / a.kt, t0 = run_first(nt, a.splits, split), t1 = run_first(nt, a.splits, split + 1);
         const int tq0 = a.q_start + qb * BLK, place = dist - (tq0 - (nt * a.kt - 1));
-        if (nt == 0 || place < 0 || dist > tq0 + BLK - 1) continue;
-        s += a.part[((int64_t)((b * a.H + h) * a.n_qb + qb) * 2 + cls) * a.span + place];
+        if (t0 == t1 || dist < tq0 - (t1 * a.kt - 1) || dist > tq0 + BLK - 1 - t0 * a.kt) continue;     // no pair of the run's
+        s += a.part[((((int64_t)b * a.H + h) * a.n_qb + qb) * a.splits + split) * 2 * a.span + (int64_t)cls * a.span + place];
     }
     red[threadIdx.x] = s;
     __syncthreads();
@@ -1423,16 +1452,31 @@ int kv_splits(const rgbd_attn_desc* d) {
     return s < (d->D == 128 ? 2 : 3) ? 1 : (int)s;
 }
 
+// Runs of keys for dq where its workgroups leave compute units idle: as many as fill the chip twice over, of at least two tiles each; with a
+// workgroup on every compute unit already, only from 32 tiles on.  us cut (with the sum of the runs) / whole: 64x64 x 2 heads of 64, one sample
+// (8 runs) 46 / 148, two samples 60 / 114; 4 x 32x32 x 4 (4 runs) 38 / 46; 8 x 16x16 x 4 (2 runs) 24 / 27; 5 x 713 x 6 of 32 (2 runs) 52 / 70;
+// line (2 runs) 154 / 175; but 8 x 32x32 x 4 of 64, 256 workgroups of 16 tiles, 43 / 41.
+int dq_splits(const rgbd_attn_desc* d) {
+    const int64_t groups = (int64_t)d->B * d->H * ceil_div(d->Lq, BLK), tiles = ceil_div(d->Lk, kt_of(d->D));
+    if (groups == 0 || (groups >= 256 && tiles < 32)) return 1;
+    int64_t s = 512 / groups;
+    if (s > tiles / 2) s = tiles / 2;
+    if (s > 64) s = 64;
+    return (int)(s < 1 ? 1 : s);
+}
+
 // Floats of the backward workspace: delta, the table's partials of `chunk` samples (PART_FLOATS at most, or one sample), what the first
 // reduction leaves of them, the runs' dk and dv.
 constexpr int64_t PART_FLOATS = 128 << 20;
-struct BwdSizes { int64_t delta, part, sums, kv; int mode, chunk, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
+struct BwdSizes { int64_t delta, part, sums, kv, dq; int mode, dq_runs, chunk, span, n_dist, d0, q_row0, q_rows, k_rows, gq, gk; };
 BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     BwdSizes z{};
     z.chunk = d->B;
     z.delta = ((int64_t)d->B * d->H * d->Lq + 3) / 4 * 4;
     const int ks = kv_splits(d);
     z.kv = ks > 1 ? (int64_t)ks * d->B * d->Hkv * d->Lk * 2 * d->D : 0;
+    z.dq_runs = dq_splits(d);
+    z.dq = z.dq_runs > 1 ? (int64_t)z.dq_runs * d->B * d->Lq * d->H * d->D : 0;
     if (!dt || d->Lq == 0 || d->Lk == 0) return z;
     const int KT = kt_of(d->D), n_qb = ceil_div(d->Lq, BLK), n_kt = ceil_div(d->Lk, KT);
     if (d->rows == 1 || (d->cols % 32 == 0 && d->q_start % d->cols == 0)) {
@@ -1447,7 +1491,7 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
     } else {
         z.mode = DT_DIAGONALS;
         z.span = n_kt * KT + BLK;
-        z.part = (int64_t)d->H * n_qb * 2 * z.span;
+        z.part = (int64_t)d->H * n_qb * z.dq_runs * 2 * z.span;
         z.d0 = d->q_start - (n_kt * KT - 1);                          // distances from there to q_start + n_qb * BLK - 1
         z.n_dist = d->q_start + n_qb * BLK - z.d0;
         z.sums = (int64_t)d->H * 2 * z.n_dist;
@@ -1507,7 +1551,7 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
 extern "C" int64_t rgbd_attention_bwd_workspace(const rgbd_attn_desc* d, int want_table) {
     if (check_desc(d, "rgbd_attention_bwd_workspace")) return -1;
     const BwdSizes z = bwd_sizes(d, want_table && d->table);
-    return z.delta + z.part + z.sums + z.kv + 4;
+    return z.delta + z.part + z.sums + z.kv + z.dq + 4;
 }
 
 extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad* g, float* workspace, void* stream) {
@@ -1550,15 +1594,18 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
         a.seg_tiles = w.tiles;
         a.win_bytes = w.win_bytes;
         const size_t lds = 4 * a.kt * 2 * d->D + dt_lds(z.mode, d->D) + w.lds;
+        a.splits = z.dq_runs;
+        a.run_floats = (int64_t)d->B * d->Lq * d->H * d->D;
+        a.runs = workspace + z.delta + z.part + z.sums + z.kv;
         for (int b0 = 0; b0 < d->B; b0 += z.chunk) {
             AttnArgs c = a;
             c.B = d->B - b0 < z.chunk ? d->B - b0 : z.chunk;
             const int64_t rows = (int64_t)b0 * a.H * a.Lq;
             c.q += b0 * a.q_sb; c.k += b0 * a.k_sb; c.v += b0 * a.v_sb; c.dq += b0 * a.dq_sb;
             c.d_o += rows * d->D; c.o += rows * d->D; c.o_lo += rows * d->D;
-            c.lse += rows; c.delta += rows;
+            c.lse += rows; c.delta += rows; c.runs += rows * d->D;
             if (c.lengths) c.lengths += b0;
-            const unsigned grid = (unsigned)c.B * a.H * a.n_qb;
+            const unsigned grid = (unsigned)c.B * a.H * a.n_qb * a.splits;
             const int rc = d->D == 32   ? launch_dq<32>(c, bias, cap, z.mode, grid, lds, s)
                            : d->D == 64 ? launch_dq<64>(c, bias, cap, z.mode, grid, lds, s)
                                         : launch_dq<128>(c, bias, cap, z.mode, grid, lds, s);
@@ -1570,6 +1617,8 @@ extern "C" int rgbd_attention_bwd(const rgbd_attn_desc* d, const rgbd_attn_grad*
             else if (z.mode == DT_DIAGONALS)
                 hipLaunchKernelGGL(attn_dist_kernel, dim3(ceil_div(z.n_dist, 64), 2 * a.H), dim3(1024), 0, s, c, sums, b0 > 0, z.n_dist, z.d0);
         }
+        if (a.splits > 1)
+            hipLaunchKernelGGL(attn_dq_sum_kernel, dim3((unsigned)((a.run_floats / 4 + 255) / 256)), dim3(256), 0, s, a, d->D);
         if (z.mode == DT_BLOCKS)
             hipLaunchKernelGGL(attn_block_bucket_kernel, dim3(a.n_buckets, a.H), dim3(256), 0, s, a, sums, g->order, g->start, z.q_row0, z.k_rows,
                                z.q_rows, z.gq, z.gk);

@@ -450,6 +450,22 @@ def test_many_samples_of_few_queries_and_runs_of_queries():
         full_check(q, k, v, None, None, do, lengths=torch.tensor([n - 7] * B, dtype=torch.int32, device=DEV))
 
 
+def test_keys_in_runs_for_the_gradient_of_queries():
+    """Few workgroups: runs of two tiles and more, lengths that leave runs empty or short, every way the table's sums are taken."""
+    for rows, cols, lq, H, Hkv, D, cap, lens in ((20, 20, 0, 2, 1, 64, 0.0, [400, 130, 0]), (32, 32, 0, 2, 2, 64, 9.0, [1024, 1]),
+                                                (1, 1000, 300, 4, 2, 128, 0.0, [999, 64]), (19, 33, 200, 2, 2, 32, 4.0, [627, 65]),
+                                                (64, 64, 100, 1, 1, 32, 0.0, [4096]), (8, 40, 0, 2, 2, 128, 0.0, None)):
+        n = rows * cols
+        lq = lq or n
+        B = len(lens) if lens else 2
+        b = buckets(rows, cols, 9)
+        q, k, v, table, do = inputs(80, B, lq, n, H, Hkv, D, b.n_buckets)
+        lengths = torch.tensor(lens, dtype=torch.int32, device=DEV) if lens else None
+        full_check(q, k, v, table, b, do, cap=cap, lengths=lengths, q_start=(n - lq) // 2)
+    q, k, v, _, do = inputs(81, 1, 300, 2000, 2, 2, 64)
+    full_check(q, k, v, None, None, do, lengths=torch.tensor([1234], dtype=torch.int32, device=DEV))
+
+
 def test_a_negative_scale_is_a_negative_query():
     b = buckets(9, 13, 7)
     q, k, v, table, do = inputs(60, 2, 117, 117, 4, 2, 64, b.n_buckets)
