@@ -45,7 +45,7 @@ struct AttnArgs {
     int B, H, Hkv, rep, Lq, Lk;
     int rows, cols, pos_cols, q_start, n_buckets;
     int kt, n_qb, n_kb, n_kt, seg_tiles, win_bytes, splits;
-    float* runs; int64_t run_floats;      // dq in runs of keys: their fp32 sums (splits, B, Lq, H, D)
+    float* runs; int64_t run_floats;      // output or dq in runs of keys: their fp32 sums (splits, B, Lq, H, D)
     int span;                             // width of a row of bias-gradient partials (distances a workgroup meets)
     float scale, cap;
 };
@@ -330,6 +330,9 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
     return a.lengths ? min(max(a.lengths[b], 0), a.Lk) : a.Lk;
 }
 
+// First of n tiles of a run.
+__device__ __forceinline__ int run_first(int n, int runs, int run) { return min(n, (n + runs - 1) / runs * run); }
+
 // ======================================================================================================= forward
 // A workgroup owns 128 queries of a head, a wave 32 of them, and streams tiles of keys and values (64 rows, 32 at head size 128) through
 // two LDS buffers: the next tile's loads run under the whole of this one's work.  What bounds it is issue, not a pipe: of the cycles of a
@@ -337,7 +340,8 @@ __device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
 // with two or three waves they overlap little.  Leaving out, one at a time, the exponentials, half of the second product, the bias reads
 // or the tiles' loads shortens it by 9 .. 12 % each; both blocks' first products ahead of the softmax change nothing.  Three workgroups
 // a compute unit at head size 64 (registers and LDS; four spill), two at 128.  32 px 50 without bias, 63 with; 128 px 360 .. 400 (690 ..
-// 760 TFLOP/s; its 512 workgroups are two a compute unit), three times its samples 850 TFLOP/s.
+// 760 TFLOP/s; its 512 workgroups are two a compute unit), three times its samples 850 TFLOP/s.  Few workgroups: the keys are cut into
+// `splits` runs, whose fp32 outputs, references and sums a second launch joins.
 // LDS: K[2] V[2] tiles | window | table of the segment's places (BIAS 1).
 // FINE: the probabilities go into the second product as three bf16 terms (24 bits): delta = do . o must be that exact where the fp32
 // gradient of the table is wanted, whose sums cancel.  Its error against 64 bits over forms of 18 to 8192 tokens: one term 5e-4, two
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
     int* at = reinterpret_cast<int*>(win + a.win_bytes);
 
     const int id = xcd_run(blockIdx.x, gridDim.x);
-    const int qb = id % a.n_qb, bh = id / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
+    const int split = id % a.splits, own = id / a.splits, qb = own % a.n_qb, bh = own / a.n_qb, h = bh % a.H, b = bh / a.H, hk = h / a.rep;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
     const int row = qb * BLK + wave * 32 + (lane & 31);
     const Frags<D> fr(lane);
@@ -363,9 +367,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
         for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
     }
     const int len = keys_of(a, b);
-    const int nt = (len + KT - 1) / KT;
-    const unsigned short* kp = a.k + b * a.k_sb + hk * a.k_sh;
-    const unsigned short* vp = a.v + b * a.v_sb + hk * a.v_sh;
+    const int nt = (len + KT - 1) / KT, t0 = run_first(nt, a.splits, split), t1 = run_first(nt, a.splits, split + 1);
+    const unsigned short* kp = a.k + b * a.k_sb + (int64_t)t0 * KT * a.k_sl + hk * a.k_sh;
+    const unsigned short* vp = a.v + b * a.v_sb + (int64_t)t0 * KT * a.v_sl + hk * a.v_sh;
 
     const int tq0 = a.q_start + qb * BLK, tq1 = a.q_start + min(qb * BLK + BLK, a.Lq) - 1;
     const int pq0 = BIAS ? pos_of(tq0, a.pos_cols) : 0, pq1 = BIAS ? pos_of(tq1, a.pos_cols) : 0;
@@ -382,11 +386,11 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
 
     Dma<D, KT> sk, sv;
     Places<BIAS> pl;
-    int seg_t = 0;                                                   // the first tile of the segment in the window
-    if (BIAS) pl.init(a, 0);
-    if (nt > 0) {
-        sk.init(kp, a.k_sl, len, smem);
-        sv.init(vp, a.v_sl, len, smem + 2 * TB);
+    int seg_t = t0;                                                  // the first tile of the segment in the window
+    if (BIAS) pl.init(a, t0 * KT);
+    if (t0 < t1) {
+        sk.init(kp, a.k_sl, len - t0 * KT, smem);
+        sv.init(vp, a.v_sl, len - t0 * KT, smem + 2 * TB);
         sk.next(a.k_sl, 0);
         sv.next(a.v_sl, 0);
         dma_wait();
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
         constexpr int P = decltype(parity)::value;
         const char* kc = smem + P * TB;
         const char* vc = smem + (2 + P) * TB;
-        if (BIAS && (t == 0 || t == seg_t + a.seg_tiles)) {
+        if (BIAS && (t == t0 || t == seg_t + a.seg_tiles)) {
             __syncthreads();                                         // every wave is done with the last window
             seg_t = t;
             pl.blk = 0;
@@ -405,7 +409,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
             Places<BIAS>::table(at, a, t * KT, n, a.Lk - 1);
         }
         __syncthreads();
-        if (t + 1 < nt) {
+        if (t + 1 < t1) {
             sk.next(a.k_sl, (P ^ 1) * TB);
             sv.next(a.v_sl, (P ^ 1) * TB);
         }
@@ -495,12 +499,23 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
         }
         dma_wait();
     };
-    for (int t = 0; t < nt; t += 2) {
+    for (int t = t0; t < t1; t += 2) {
         tile(t, std::integral_constant<int, 0>{});
-        if (t + 1 < nt) tile(t + 1, std::integral_constant<int, 1>{});
+        if (t + 1 < t1) tile(t + 1, std::integral_constant<int, 1>{});
     }
     l = other_half_sum(l);
     if (row >= a.Lq) return;
+    if (a.splits > 1) {
+        const int64_t at_row = ((int64_t)b * a.Lq + row) * a.H + h;
+        float* p = a.runs + split * a.run_floats + at_row * D + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<f32x4*>(p + 32 * d + 8 * g) = f32x4{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        if (half == 0) *reinterpret_cast<f32x2_t*>(a.part + 2 * (split * (a.run_floats / D) + at_row)) = f32x2_t{m, l};
+        return;
+    }
     const float il = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);       // no key: 0; a NaN stays one
     if (a.lse && half == 0) a.lse[(int64_t)bh * a.Lq + row] = l == 0.f ? 0.f : m + __builtin_amdgcn_logf(l);
     const int64_t ob = (((int64_t)b * a.Lq + row) * a.H + h) * D + 4 * half;
@@ -518,6 +533,48 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
                 *reinterpret_cast<u32x2*>(a.out_lo + ob + 32 * d + 8 * g) = r;
             }
         }
+}
+
+// Output from the runs' sums, references and probabilities (part: (splits, B, Lq, H, 2)): four values a thread, grid
+// (sample, query, head, D / 4) / 256.
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int D) {
+    const int64_t e = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x), row = e / D;
+    if (e >= a.run_floats) return;
+    const int64_t rows = a.run_floats / D;
+    float m = NEG_INF, l = 0.f;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    auto of_run = [&](int i) { return *reinterpret_cast<const f32x2_t*>(a.part + 2 * (min(i, a.splits - 1) * rows + row)); };
+    for (int i0 = 0; i0 < a.splits; i0 += 4) {
+        f32x2_t ml[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ml[j] = of_run(i0 + j);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ml[j][1] != 0.f) m = fmaxf(m, ml[j][0]);              // (a run without keys has no reference; one of NaN has)
+    }
+    for (int i0 = 0; i0 < a.splits; i0 += 4) {
+        f32x2_t ml[4];
+        f32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            ml[j] = of_run(i0 + j);
+            v[j] = *reinterpret_cast<const f32x4*>(a.runs + min(i0 + j, a.splits - 1) * a.run_floats + e);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i0 + j >= a.splits || ml[j][1] == 0.f) continue;
+            const float al = __builtin_amdgcn_exp2f(ml[j][0] - m);
+            l += ml[j][1] * al;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] += v[j][k] * al;
+        }
+    }
+    const float il = l > 0.f ? 1.f / l : l;                          // no key: 0; a NaN stays one
+    const int64_t h = row % a.H, bq = row / a.H, b = bq / a.Lq, qi = bq - b * a.Lq;
+    if (a.lse && e % D == 0) a.lse[(b * a.H + h) * a.Lq + qi] = l == 0.f ? 0.f : m + __builtin_amdgcn_logf(l);
+    *reinterpret_cast<u32x2*>(a.out + e) = u32x2{pack_bf16x2(s[0] * il, s[1] * il), pack_bf16x2(s[2] * il, s[3] * il)};
+    if (a.out_lo)
+        *reinterpret_cast<u32x2*>(a.out_lo + e) = u32x2{low_half(s[0] * il) | low_half(s[1] * il) << 16, low_half(s[2] * il) | low_half(s[3] * il) << 16};
 }
 
 // ======================================================================================================= forward, few rows
@@ -762,9 +819,6 @@ constexpr int block_rows(int D) { return D == 128 ? 16 : 32; }       // (16: a b
 constexpr int block_floats(int D) { return 32 + block_rows(D) * BS; }
 constexpr int dt_lds(int dt, int D) { return dt == DT_BLOCKS ? 4 * block_floats(D) * 4 : dt == DT_DIAGONALS ? kt_of(D) * BLK * 4 : 0; }
 
-// First of n tiles of a run.
-__device__ __forceinline__ int run_first(int n, int runs, int run) { return min(n, (n + runs - 1) / runs * run); }
-
 template <int D, int BIAS, bool CAP, int DT>
 __global__ __launch_bounds__(256, D == 32 ? 3 : 2) void attn_dq_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -983,10 +1037,15 @@ __global__ __launch_bounds__(256) void attn_dq_sum_kernel(AttnArgs a, int D) {
     const int64_t e = 4 * ((int64_t)blockIdx.x * 256 + threadIdx.x);
     if (e >= a.run_floats) return;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < a.splits; ++i) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.runs + i * a.run_floats + e);
+    for (int i0 = 0; i0 < a.splits; i0 += 4) {
+        f32x4 v[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] += v[k];
+        for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const f32x4*>(a.runs + min(i0 + j, a.splits - 1) * a.run_floats + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (i0 + j < a.splits)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[k] += v[j][k];
     }
     const int64_t row = e / D / a.H, b = row / a.Lq;
     unsigned short* o = a.dq + b * a.dq_sb + (row - b * a.Lq) * a.dq_sl + e / D % a.H * a.dq_sh + e % D;
@@ -1452,18 +1511,21 @@ int kv_splits(const rgbd_attn_desc* d) {
     return s < (d->D == 128 ? 2 : 3) ? 1 : (int)s;
 }
 
-// Runs of keys for dq where its workgroups leave compute units idle: as many as fill the chip twice over, of at least two tiles each; with a
-// workgroup on every compute unit already, only from 32 tiles on.  us cut (with the sum of the runs) / whole: 64x64 x 2 heads of 64, one sample
-// (8 runs) 46 / 148, two samples 60 / 114; 4 x 32x32 x 4 (4 runs) 38 / 46; 8 x 16x16 x 4 (2 runs) 24 / 27; 5 x 713 x 6 of 32 (2 runs) 52 / 70;
-// line (2 runs) 154 / 175; but 8 x 32x32 x 4 of 64, 256 workgroups of 16 tiles, 43 / 41.
-int dq_splits(const rgbd_attn_desc* d) {
+// Runs of keys for the forward pass and dq where their workgroups leave compute units idle: as many as fill the chip twice over, of at least
+// `least` tiles each (6 forward, 2 for dq); with a workgroup on every compute unit already, only from 32 tiles on.  us cut (with the launch
+// that joins the runs) / whole, forward, dq: 64x64 x 2 heads of 64, one sample (8 runs) 46 / 130, 46 / 148, two samples (4 runs) 55 / 100,
+// 60 / 114; 4 x 32x32 x 4 of 64, capped (2 and 4 runs) 30 / 39, 38 / 46; 5 x 713 x 6 of 32 (2 runs) 30 / 32, 52 / 70; line (2 runs) 144 / 166,
+// 153 / 175; 8 x 16x16 x 4 of 64 (2 runs for dq) 24 / 27; but 8 x 32x32 x 4 of 64, 256 workgroups of 16 tiles, dq 43 / 41.
+int key_runs(const rgbd_attn_desc* d, int least) {
     const int64_t groups = (int64_t)d->B * d->H * ceil_div(d->Lq, BLK), tiles = ceil_div(d->Lk, kt_of(d->D));
     if (groups == 0 || (groups >= 256 && tiles < 32)) return 1;
     int64_t s = 512 / groups;
-    if (s > tiles / 2) s = tiles / 2;
+    if (s > tiles / least) s = tiles / least;
     if (s > 64) s = 64;
     return (int)(s < 1 ? 1 : s);
 }
+int fwd_splits(const rgbd_attn_desc* d) { return key_runs(d, 6); }
+int dq_splits(const rgbd_attn_desc* d) { return key_runs(d, 2); }
 
 // Floats of the backward workspace: delta, the table's partials of `chunk` samples (PART_FLOATS at most, or one sample), what the first
 // reduction leaves of them, the runs' dk and dv.
@@ -1509,8 +1571,9 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
 extern "C" int64_t rgbd_attention_fwd_workspace(const rgbd_attn_desc* d) {
     if (check_desc(d, "rgbd_attention_fwd_workspace")) return -1;
     if (d->B == 0 || d->Lq == 0) return 0;
-    const int runs = few_splits(d);
-    return runs > 1 ? (int64_t)d->B * d->Hkv * runs * 32 * (d->D + 2) : 0;
+    const int few = few_splits(d), runs = few ? 1 : fwd_splits(d);
+    if (few > 1) return (int64_t)d->B * d->Hkv * few * 32 * (d->D + 2);
+    return runs > 1 ? (int64_t)runs * d->B * d->Lq * d->H * (d->D + 2) : 0;
 }
 
 extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, float* workspace, void* stream) {
@@ -1537,13 +1600,19 @@ extern "C" int rgbd_attention_fwd(const rgbd_attn_desc* d, void* o, void* o_lo, 
     RGBD_REQUIRE(bias == 0 || d->Lk == 0 || w.tiles > 0, "rgbd_attention_fwd: the bias of one tile does not fit (%d x %d grid)", a.rows, a.cols);
     a.seg_tiles = w.tiles;
     a.win_bytes = w.win_bytes;
+    a.splits = fwd_splits(d);
+    a.run_floats = (int64_t)d->B * d->Lq * d->H * d->D;
+    a.runs = workspace;
+    a.part = workspace + a.splits * a.run_floats;
+    RGBD_REQUIRE(a.splits == 1 || (workspace && ((uintptr_t)workspace & 15) == 0), "rgbd_attention_fwd: null or unaligned workspace");
     const size_t lds = 4 * a.kt * 2 * d->D + w.lds;
-    const unsigned grid = (unsigned)a.B * a.H * a.n_qb;
+    const unsigned grid = (unsigned)a.B * a.H * a.n_qb * a.splits;
     const bool fine = d->fine && bias;
     const int rc = d->D == 32   ? launch_fwd<32>(a, bias, cap, fine, grid, lds, s)
                    : d->D == 64 ? launch_fwd<64>(a, bias, cap, fine, grid, lds, s)
                                 : launch_fwd<128>(a, bias, cap, fine, grid, lds, s);
     if (rc) return rc;
+    if (a.splits > 1) hipLaunchKernelGGL(attn_join_kernel, dim3((unsigned)((a.run_floats / 4 + 255) / 256)), dim3(256), 0, s, a, d->D);
     RGBD_CHECK_LAUNCH("rgbd_attention_fwd");
     return 0;
 }

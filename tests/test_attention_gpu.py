@@ -450,7 +450,7 @@ def test_many_samples_of_few_queries_and_runs_of_queries():
         full_check(q, k, v, None, None, do, lengths=torch.tensor([n - 7] * B, dtype=torch.int32, device=DEV))
 
 
-def test_keys_in_runs_for_the_gradient_of_queries():
+def test_keys_in_runs():
     """Few workgroups: runs of two tiles and more, lengths that leave runs empty or short, every way the table's sums are taken."""
     for rows, cols, lq, H, Hkv, D, cap, lens in ((20, 20, 0, 2, 1, 64, 0.0, [400, 130, 0]), (32, 32, 0, 2, 2, 64, 9.0, [1024, 1]),
                                                 (1, 1000, 300, 4, 2, 128, 0.0, [999, 64]), (19, 33, 200, 2, 2, 32, 4.0, [627, 65]),
@@ -462,6 +462,15 @@ def test_keys_in_runs_for_the_gradient_of_queries():
         q, k, v, table, do = inputs(80, B, lq, n, H, Hkv, D, b.n_buckets)
         lengths = torch.tensor(lens, dtype=torch.int32, device=DEV) if lens else None
         full_check(q, k, v, table, b, do, cap=cap, lengths=lengths, q_start=(n - lq) // 2)
+    # scores far apart between the runs, rows of which one run has no key or all
+    b = buckets(1, 1000, 9, 500)
+    q, k, v, table, do = inputs(82, 1, 1000, 1000, 1, 1, 64, b.n_buckets)
+    for far in (300.0, -300.0, -math.inf):
+        t = table.clone()
+        t[0, 0] += far
+        t[0, 8] -= far if far > -math.inf else -7.0
+        got = run(q, k, v, t, b, do)
+        check(got, definition(q, k, v, t, b, do, None, 0.0, None, 0, True), ["o", "dq", "dk", "dv", "dtable"])
     q, k, v, _, do = inputs(81, 1, 300, 2000, 2, 2, 64)
     full_check(q, k, v, None, None, do, lengths=torch.tensor([1234], dtype=torch.int32, device=DEV))
 
