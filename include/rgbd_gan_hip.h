@@ -609,7 +609,7 @@ int rgbd_group_norm_bwd(const void* x, const void* dy, const float* gamma, const
  *   rows == 1, or cols <= 1024.  cap 0 or in [1e-12, 1e12], |scale| in [1e-12, 1e12], token strides and H D below 2^24.
  * o, o_lo (B, Lq, H, D) contiguous bf16: the output and (may be NULL) the low halves of its fp32 values; lse (B, H, Lq) fp32 (may be NULL):
  *   log2 of the row's sum of exp, in units of log2 -- o_lo and lse are what the backward pass needs.  fine != 0: the probabilities
- *   enter the second product with 16 bits instead of 8, which the table's gradient needs to be exact to fp32's last digits. */
+ *   enter the second product with 24 bits instead of 8, which the table's gradient needs to be exact to fp32's last digits. */
 typedef struct {
     const void *q, *k, *v;
     int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh;
