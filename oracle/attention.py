@@ -1,5 +1,5 @@
-"""Group norm and grid attention from their definitions, in float64 torch (CPU or GPU).  Test infrastructure only: the checker of
-rgbd_gan_amd.functional.group_norm / attention.  Differentiable by autograd; `attention_parts` also returns the matrices whose
+"""Group norm and grid attention from their definitions, in float64 torch (CPU or GPU).  Test infrastructure only: what the tests hold
+rgbd_gan_amd.functional.group_norm / attention against.  Differentiable by autograd; `attention_parts` also returns the matrices whose
 sums bound what the kernels' roundings can do (tests derive their tolerances from them)."""
 import math
 
