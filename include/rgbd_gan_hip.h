@@ -607,6 +607,8 @@ int rgbd_group_norm_bwd(const void* x, const void* dy, const float* gamma, const
  *   (row_i - row_j + rows - 1) * (2 cols - 1) + (col_i - col_j + cols - 1);  map (2 rows - 1)(2 cols - 1) int32 bucket numbers
  *   (clamped to [0, n_buckets)), table (H, n_buckets) fp32, values at or below -1e30 leaving their offsets out like -inf.
  *   rows == 1, or cols <= 1024.  cap 0 or in [1e-12, 1e12], |scale| in [1e-12, 1e12], token strides and H D below 2^24.
+ * Scores of any size; |v| below 1e29: the output is summed over the keys, with a row's probabilities at a sum of at most 2^24, before it is
+ *   divided by their sum.
  * o, o_lo (B, Lq, H, D) contiguous bf16: the output and (may be NULL) the low halves of its fp32 values; lse (B, H, Lq) fp32 (may be NULL):
  *   log2 of the row's sum of exp, in units of log2 -- o_lo and lse are what the backward pass needs.  fine != 0: the probabilities
  *   enter the second product with 24 bits instead of 8, which the table's gradient needs to be exact to fp32's last digits. */

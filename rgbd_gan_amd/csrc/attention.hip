@@ -34,6 +34,11 @@ constexpr int WIN_PAD = 4;
 constexpr int WIN_FWD = 20480, WIN_DQ = 10240;
 constexpr float NO_ROW = 0x1p100f;          // log2-sum-exp of a row that is not there: p = exp2(x - 2^100) = 0 for every finite x
 constexpr float NEG_INF = -__builtin_inff();
+// Where a row's sum of probabilities may lie before the forward pass moves its reference.  The output is summed as p v before the division by that
+// sum, so a sum of S takes S from the range of |v| that fp32 can add up: with [2^-10, 2^24], 2^24 being what the largest number of keys reaches
+// next to a reference at their maximum, finite outputs stay finite and keep bf16's digits for |v| in [1e-27, 1e29] (runs of keys joined
+// included), and scores of order 1 over 2^14 keys (a sum near 2^15) never leave it.
+constexpr float SUM_LOW = 0x1p-10f, SUM_HIGH = 0x1p24f;
 
 struct AttnArgs {
     const unsigned short *q, *k, *v, *d_o, *o, *o_lo;
@@ -378,9 +383,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = splat(0.f);
-    // The softmax's reference m: probabilities are exp2(x - m).  fp32 sums and bf16 operands keep their digits at any scale, so m stays
-    // 0 while the sums stay between 2^-80 and 2^60, and no maximum is looked for; a row that leaves this range takes its block's
-    // maximum as m (and scales what it has).
+    // The softmax's reference m: probabilities are exp2(x - m).  m stays 0, and no maximum is looked for, while a row's sum stays between
+    // SUM_LOW and SUM_HIGH; a row that leaves this range takes as m what makes its sum about 1 (its log-sum-exp so far, or the block's
+    // maximum where that is larger) and scales what it has.
     float m = 0.f, l = 0.f;
     bool moved = false;                                              // (of the wave) some m is not 0
 
@@ -448,9 +453,9 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
                 sum += x[i];
             }
             float ln = l + sum;
-            if (__any(!(ln > 0x1p-80f && ln < 0x1p60f))) {           // (a NaN comes here too, and stays one)
+            if (__any(!(ln > SUM_LOW && ln < SUM_HIGH))) {           // (a NaN comes here too, and stays one)
                 const float both = other_half_sum(ln);
-                const bool bad = !(both > 0x1p-80f && both < 0x1p60f);
+                const bool bad = !(both > SUM_LOW && both < SUM_HIGH);
                 if (__any(bad)) {
                     kf.load(fr, kc, 32 * u);
                     x = kf.times(qf, splat(0.f));
@@ -460,7 +465,7 @@ __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_
                     for (int i = 0; i < 16; ++i) top = fmaxf(top, x[i]);
                     top = other_half_max(top);
                     const float have = other_half_sum(l);
-                    float mn = have > 0.f ? fmaxf(m, top) : top;
+                    float mn = have > 0.f ? fmaxf(m + __builtin_amdgcn_logf(have), top) : top;
                     if (!bad || mn == NEG_INF) mn = m;
                     const float al = have > 0.f ? __builtin_amdgcn_exp2f(m - mn) : (have == 0.f ? 0.f : have);
                     m = mn;

@@ -1806,7 +1806,9 @@ def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=No
     head h // (H // Hkv)); scale defaults to D ** -0.5, cap 0 leaves scores uncapped; lengths (B,) int32 on the device.
     table (H, n_buckets) fp32 with `buckets` (RelativeBuckets): the bias table[h, bucket of the offset], query i at token
     q_start + i of the grid, key j at token j; values at or below -1e30 (and -inf) leave their offsets out.  A grid of more than one
-    row has at most 1024 columns.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table."""
+    row has at most 1024 columns.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table.
+
+    Scores of any size; values within 1e29 (beyond, sums over keys may overflow although their average would not)."""
     spec = (None if scale is None else float(scale), float(cap or 0.0), int(q_start))
     q, k, v = _readable(q), _readable(k), _readable(v)
     table = table.contiguous() if table is not None else None

@@ -543,3 +543,15 @@ def test_offsets_beyond_two_to_the_31():
     a, c = run(*views, None, None, do), run(q, k, v, None, None, do)
     for n in a:
         assert torch.equal(a[n], c[n]), n
+
+
+@pytest.mark.parametrize("far,size", [(35.0, 1e22), (-50.0, 1e-18), (0.0, 1e29), (0.0, 1e-27), (16.0, 1e29), (-6.0, 1e-27)])
+def test_values_far_from_one(far, size):
+    """Scores and values both away from 1: the output is finite and keeps its digits, whatever the sum of the exponentials times a value
+    would be.  The whole form, keys in runs, few queries."""
+    for rows, cols, lq, H, Hkv, D in ((9, 9, 81, 2, 1, 64), (1, 1000, 300, 2, 1, 128), (1, 3000, 5, 2, 1, 32)):
+        n = rows * cols
+        b = buckets(rows, cols, 9)
+        q, k, v, table, do = inputs(90, 2, lq, n, H, Hkv, D, b.n_buckets)
+        lengths = torch.tensor([n, n - 13], dtype=torch.int32, device=DEV)
+        full_check(q, k, (size * v.float()).to(BF16), table + far, b, do, lengths=lengths, q_start=n - lq)
