@@ -588,7 +588,8 @@ int rgbd_adam_clip_multi(float* p, float* g, float* m, float* v, int64_t n,
  * values (biased, like the instance norm above), y = act((x - mean) * rstd * gamma[c] + beta[c]).
  *   dtype 0: x, y, dy, dx bf16; 1: fp32.  gamma, beta, dgamma, dbeta, mean, rstd fp32; mean, rstd (B, groups).
  *   act 0: none; 1: leaky ReLU (slope for z <= 0); 2: SiLU z / (1 + exp(-z)).
- *   workspace: rgbd_group_norm_workspace floats, uninitialised (0: may be NULL).  Sums are ordered by the shape alone (no atomics).
+ *   workspace: rgbd_group_norm_workspace floats, uninitialised (0: may be NULL).  Sums are ordered by the shape and
+ *   by whether every map of the call is 16-byte aligned (no atomics).
  *   C: at most 8192 (bf16) / 4096 (fp32); 1024 where C is no multiple of a 16-byte vector or a buffer is not 16-byte aligned.
  * _bwd writes (does not accumulate) dx, dgamma, dbeta; B or N 0: dgamma, dbeta = 0. */
 int64_t rgbd_group_norm_workspace(int B, int N, int C, int groups, int dtype, int backward);   /* floats; -1: bad sizes */

@@ -19,7 +19,7 @@
 // 16 and 8 vectors a thread instead of 8 and 4 spill; four workgroups a compute unit for the slabs' sums.
 // Statistics never come from sums of squares: a thread's eight pixels give a mean and a sum of squared deviations, and these
 // pairs are merged (Chan, Golub, LeVeque 1979), so a mean far from zero costs no digits.  Everything is summed in fp32 in an
-// order that depends on the shape alone: results are the same from run to run.
+// order that depends on the shape (and on whether the maps are 16-byte aligned) alone: results are the same from run to run.
 #include "common.h"
 
 namespace {

@@ -1692,13 +1692,21 @@ class _GroupNorm(torch.autograd.Function):
     @_once
     def backward(ctx, dy):
         x, gamma, beta, stats = ctx.saved_tensors
-        return *kernels.group_norm_bwd(x, dy.contiguous(), gamma, beta, stats, *ctx.spec), None, None, None, None
+        return *kernels.group_norm_bwd(x, _vectors(dy), gamma, beta, stats, *ctx.spec), None, None, None, None
+
+
+def _vectors(t):
+    """t contiguous and, where a pixel's channels are whole 16-byte vectors, 16-byte aligned: at another address the kernels would go value by
+    value, in another order of sums and with fewer channels at most."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 and t.dim() > 1 and t.shape[-1] * t.element_size() % 16 == 0 else t
 
 
 def group_norm(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
     """act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and variance over each sample's groups of C / groups neighbouring
-    channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu"."""
-    x, gamma, beta = x.contiguous(), gamma.contiguous(), beta.contiguous()
+    channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu".  At most
+    65535 samples and 8192 (bf16) or 4096 (fp32) channels, 1024 where C is no multiple of 8 or 4."""
+    x, gamma, beta = _vectors(x), gamma.contiguous(), beta.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
         return _GroupNorm.apply(x, gamma, beta, groups, eps, act, slope)
     return kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)[0]

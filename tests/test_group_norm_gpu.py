@@ -186,3 +186,22 @@ def test_group_norm_refuses_second_derivatives_and_wide_scalar_maps():
     wide = torch.zeros(1, 2, 1026, device=DEV)
     with pytest.raises(RuntimeError, match="channels"):
         Fn.group_norm(wide, torch.ones(1026, device=DEV), torch.zeros(1026, device=DEV), 2)
+
+
+@pytest.mark.parametrize("shape,groups,dtype", [((2, 3, 5, 2048), 4, BF16), ((2, 3, 5, 2048), 4, F32), ((2, 40, 40, 64), 8, BF16), ((3, 7, 9, 12), 3, F32)],
+                         ids=lambda s: str(s).replace(" ", ""))
+def test_tensors_at_odd_addresses(shape, groups, dtype):
+    """x, the output gradient or both at an address that is not 16-byte aligned: every width that is taken elsewhere is taken, and the
+    numbers are the same bit for bit."""
+    x, gamma, beta, dy = inputs(22, shape, dtype)
+    base = check(x, gamma, beta, dy, groups, "silu")
+
+    def odd(t):
+        buf = torch.empty(t.numel() + 8, dtype=dtype, device=DEV)
+        out = buf[1:1 + t.numel()].view(t.shape)
+        out.copy_(t)
+        assert out.is_contiguous() and out.data_ptr() % 16
+        return out
+
+    for a, d in ((x, odd(dy)), (odd(x), dy), (odd(x), odd(dy))):
+        assert all(torch.equal(p, q) for p, q in zip(base, run(a, gamma, beta, d, groups, "silu")))
