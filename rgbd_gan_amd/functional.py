@@ -17,6 +17,7 @@ import os
 import numpy as np
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 
 from . import kernels
 
@@ -1680,6 +1681,18 @@ def _once(backward):
     return run
 
 
+def _recorded(*tensors):
+    """Whether a call goes through its autograd Function: a graph is wanted, or inside a forward-mode level, where the Function refuses
+    tangents (past it they would be dropped without a word)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gamma, beta, groups, eps, act, slope):
@@ -1707,7 +1720,7 @@ def group_norm(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
     channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu".  At most
     65535 samples and 8192 (bf16) or 4096 (fp32) channels, 1024 where C is no multiple of 8 or 4."""
     x, gamma, beta = _vectors(x), gamma.contiguous(), beta.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad or beta.requires_grad):
+    if _recorded(x, gamma, beta):
         return _GroupNorm.apply(x, gamma, beta, groups, eps, act, slope)
     return kernels.group_norm_fwd(x, gamma, beta, groups, eps, act, slope)[0]
 
@@ -1821,7 +1834,7 @@ def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=No
     q, k, v = _readable(q), _readable(k), _readable(v)
     table = table.contiguous() if table is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (table is not None and table.requires_grad)):
+    if _recorded(q, k, v, table):
         return _Attention.apply(q, k, v, table, lengths, buckets, spec)
     return kernels.attention_fwd(kernels.AttnOperands.of(q, k, v), table, buckets, lengths, *spec)[0]
 
@@ -1838,6 +1851,6 @@ def attention_packed(qkv, heads, kv_heads=None, table=None, buckets=None, scale=
     qkv = _readable(qkv)
     table = table.contiguous() if table is not None else None
     lengths = lengths.contiguous() if lengths is not None else None
-    if torch.is_grad_enabled() and (qkv.requires_grad or (table is not None and table.requires_grad)):
+    if _recorded(qkv, table):
         return _AttentionPacked.apply(qkv, table, lengths, buckets, (heads, kv_heads), spec)
     return kernels.attention_fwd(kernels.AttnOperands.packed(qkv, heads, kv_heads), table, buckets, lengths, *spec)[0]

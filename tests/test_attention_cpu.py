@@ -197,3 +197,34 @@ def test_self_attention_option():
     for arch in ("dcgan", "deepvoxels"):
         with pytest.raises(AssertionError, match="self_attention"):
             setup_generator(Config(dict(generator_architecture=arch, ch=256, self_attention=32)), "cpu")
+
+
+# ------------------------------------------------------------------------------------------------ derivatives that are not there
+def test_forward_mode_derivatives_are_refused(monkeypatch):
+    """A tangent on any input raises, whether or not gradients are recorded; without one a dual level changes nothing.  (The kernels'
+    wrappers are replaced: the refusal needs no GPU.)"""
+    import torch.autograd.forward_ad as ad
+    from rgbd_gan_amd import functional as Fn
+    from rgbd_gan_amd import kernels
+    monkeypatch.setattr(kernels, "group_norm_fwd", lambda x, *a: (torch.empty_like(x), torch.empty(4)))
+    monkeypatch.setattr(kernels, "attention_fwd", lambda op, *a, **kw: (torch.empty_like(op.tensors[0]),) * 3)
+    x, g, q = bf(2, 3, 16), torch.ones(16), bf(2, 4, 2, 64)
+    b = log_map(2, 2)
+    table = torch.zeros(2, b.n_buckets)
+    calls = {
+        "x": (x, lambda t: Fn.group_norm(t, g, g, 4)), "gamma": (g, lambda t: Fn.group_norm(x, t, g, 4)), "beta": (g, lambda t: Fn.group_norm(x, g, t, 4)),
+        "q": (q, lambda t: Fn.attention(t, q, q)), "k": (q, lambda t: Fn.attention(q, t, q)), "v": (q, lambda t: Fn.attention(q, q, t)),
+        "table": (table, lambda t: Fn.attention(q, q, q, t, b)), "packed": (bf(2, 4, 384), lambda t: Fn.attention_packed(t, 2)),
+        "packed table": (table, lambda t: Fn.attention_packed(bf(2, 4, 384), 2, table=t, buckets=b)),
+    }
+    for name, (t, call) in calls.items():
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad):
+                with ad.dual_level():
+                    call(t)
+                    with pytest.raises((RuntimeError, NotImplementedError)):
+                        call(ad.make_dual(t, torch.ones_like(t)))
+                        pytest.fail(f"{name}: the tangent was dropped")
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    torch.func.jvp(call, (t,), (torch.ones_like(t),))
+                    pytest.fail(f"{name}: the tangent was dropped")
