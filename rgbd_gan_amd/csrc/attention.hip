@@ -1563,9 +1563,9 @@ BwdSizes bwd_sizes(const rgbd_attn_desc* d, bool dt) {
         z.n_dist = d->q_start + n_qb * BLK - z.d0;
         z.sums = (int64_t)d->H * 2 * z.n_dist;
     }
-    // (a 64 x 64 map's partials are 4 MB a sample and head; from 512 MB on dq runs over as many samples at a time as stay below)
-    z.chunk = (int)((PART_FLOATS + z.part - 1) / z.part);
-    if (z.chunk > d->B) z.chunk = d->B;
+    // (a 64 x 64 map's partials are 4 MB a sample and head; above 512 MB dq runs over as many samples at a time as fit in that, one at least)
+    const int64_t fit = z.part < PART_FLOATS ? PART_FLOATS / z.part : 1;
+    z.chunk = fit < d->B ? (int)fit : d->B;
     z.part *= z.chunk;
     z.sums = (z.sums + 3) / 4 * 4;
     return z;

@@ -199,6 +199,25 @@ def test_self_attention_option():
             setup_generator(Config(dict(generator_architecture=arch, ch=256, self_attention=32)), "cpu")
 
 
+def test_partial_sums_of_the_table_stay_below_their_limit():
+    """The table gradient's partial sums take 512 MB, or what one sample takes where that is more: workspace floats of a batch against
+    those of one sample, whatever the batch (the rest of the difference is delta and runs of keys or queries, which want_table = 0 has too)."""
+    from rgbd_gan_amd import _lib, kernels
+    lib = _lib.load()
+    for rows, cols, H, D in ((128, 128, 6, 64), (64, 64, 8, 32), (100, 100, 3, 64), (63, 65, 32, 32), (1, 20000, 2, 128)):
+        d = kernels._AttnDesc()
+        d.H, d.Hkv, d.Lq, d.Lk, d.D, d.scale, d.table, d.map = H, H, rows * cols, rows * cols, D, 0.125, 16, 16
+        d.rows, d.cols, d.n_buckets = rows, cols, 9
+
+        def floats(B):
+            d.B = B
+            return lib.rgbd_attention_bwd_workspace(ctypes.byref(d), 1) - lib.rgbd_attention_bwd_workspace(ctypes.byref(d), 0)
+
+        one = floats(1)                                          # partials and what the first reduction leaves: at most 16 a head and token
+        for B in (2, 3, 5, 18, 40):
+            assert 0 < floats(B) <= max((128 << 20) + 16 * H * rows * cols, one), (rows, cols, H, B, floats(B), one)
+
+
 # ------------------------------------------------------------------------------------------------ derivatives that are not there
 def test_forward_mode_derivatives_are_refused(monkeypatch):
     """A tangent on any input raises, whether or not gradients are recorded; without one a dual level changes nothing.  (The kernels'
