@@ -555,3 +555,55 @@ def test_values_far_from_one(far, size):
         q, k, v, table, do = inputs(90, 2, lq, n, H, Hkv, D, b.n_buckets)
         lengths = torch.tensor([n, n - 13], dtype=torch.int32, device=DEV)
         full_check(q, k, (size * v.float()).to(BF16), table + far, b, do, lengths=lengths, q_start=n - lq)
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("keys", [1, 2, 5])
+def test_the_learned_tables_forward_pass_keeps_fp32_digits(keys, D):
+    """With a learned table o and its low half are one fp32 number, and the probabilities enter its product in three bf16 terms.  Queries
+    of zero leave the bias, within +-1, as the score.  A term leaves U of what it rounds, so three leave 2^-24 of a probability; the
+    product adds at most 15 terms (2^-24 each), then the division, its product and the low half: within 2^-19 of sum p |v|, and es, the
+    scores' share (2 x 2^-22 |bias| + 2^-20).  Two terms would leave up to 2^-16.  One key: o is v, and its table's gradient, do . v - do . o,
+    is 0; do has one channel, so that dp is exact and delta o's error."""
+    from rgbd_gan_amd import functional as Fn
+    from rgbd_gan_amd import kernels
+    N, H = 200, 4
+    b = Fn.RelativeBuckets(np.arange(2 * N - 1)[None, :], device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(91)
+    q = torch.zeros(2, N, H, D, device=DEV, dtype=BF16)
+    k, v = (torch.randn(2, keys, H, D, generator=g, device=DEV).to(BF16) for _ in range(2))
+    table = 2 * torch.rand(H, b.n_buckets, generator=g, device=DEV) - 1
+    o, lo, _ = kernels.attention_fwd(kernels.AttnOperands.of(q, k, v), table, b, keep=True, fine=True)
+    whole = ((o.view(torch.int16).to(torch.int32) << 16) + lo.view(torch.int16).to(torch.int32)).view(torch.float32).to(F64)
+    want, p, _, _, _, vr = ref.attention_parts(q.to(F64), k.to(F64), v.to(F64), table.to(F64), b.map.reshape(1, -1).long())
+    tol = (2 * 2.0 ** -22 + 2.0 ** -20 + 2.0 ** -19) * torch.matmul(p, vr.abs()).permute(0, 2, 1, 3)
+    worst = float(((whole - want).abs() / tol).max())
+    assert worst <= 1.0, f"{worst:.3f} of the tolerance"
+    if keys == 1:
+        do = torch.zeros_like(q)
+        do[0, :, :, 3] = torch.randn(N, H, generator=g, device=DEV).to(BF16)
+        got = run(q, k, v, table, b, do)["dtable"]
+        first = N - 1                                            # query i, key 0: offset i
+        bound = (2 * 2.0 ** -22 + 2.0 ** -20 + 2.0 ** -19 + 2.0 ** -23) * (do[0, :, :, 3].to(F64).abs() * v[0, :, :, 3].to(F64).abs()).T
+        assert float((got[:, first:].to(F64).abs() / bound.clamp_min(1e-30)).max()) <= 1.0
+        assert float(got[:, :first].abs().max()) == 0.0
+
+
+@pytest.mark.parametrize("rows,cols,lq,B,H,Hkv,D,cap", [(32, 32, 0, 3, 4, 4, 64, 0.0), (64, 64, 0, 1, 2, 2, 64, 30.0), (23, 31, 0, 3, 6, 2, 32, 20.0),
+                                                        (1, 1500, 0, 2, 4, 2, 128, 0.0), (1, 3000, 5, 2, 4, 2, 64, 0.0), (16, 16, 0, 4, 4, 4, 64, 50.0)])
+def test_the_tables_gradient_against_64_bits(rows, cols, lq, B, H, Hkv, D, cap):
+    """dtable in relative 2-norm, by blocks, by diagonals, for few queries.  A pair's ds is off by independent roundings of 2^-24: the
+    square root of D of them in each product, some 8 more on the way (bias, cap, exponential, delta), of magnitudes |dp| + |delta| up to
+    twice ds: (sqrt(128) + 8) 2^-24 x 2 < 2^-18.5 of it, and sums of independent errors keep that ratio.  One bf16 term instead of three
+    gives 5e-4."""
+    n = rows * cols
+    b = buckets(rows, cols, 15, 64)
+    q, k, v, table, do = inputs(92, B, lq or n, n, H, Hkv, D, b.n_buckets)
+    got = run(q, k, v, table, b, do, cap=cap, q_start=n - (lq or n))["dtable"].to(F64)
+    m = b.map.reshape(2 * rows - 1, 2 * cols - 1).long()
+    leaf = table.to(F64).requires_grad_(True)
+    o = ref.attention(*(t.to(F64) for t in (q, k, v)), leaf, m, cap=cap, q_start=n - (lq or n))
+    (want,) = torch.autograd.grad(o, leaf, do.to(F64))
+    err = float((got - want).norm() / want.norm())
+    print(f"dtable {rows}x{cols} lq={lq} D={D} cap={cap}: {err:.2e}", flush=True)
+    assert err <= 2.0 ** -18.5
