@@ -12,8 +12,10 @@
 // operand), so a lane holds one query and 16 of its keys: row maximum and sum need one exchange between lane l and l + 32,
 // the rescaling of the output is one factor a lane, and the 16 probabilities are, packed to bf16, the B operand of the second
 // product as they stand (its K order follows the accumulator's: 4 keys of one half, 4 of the other), while the A operand comes
-// out of LDS through the transposing read.  Probabilities and score gradients are rounded to bf16 only as operands of these
-// products; maxima, sums, statistics and the table's gradient stay in fp32.
+// out of LDS through the transposing read.  Probabilities and score gradients are rounded to bf16 as operands of these products, which
+// makes o, dq, dk and dv two bf16 roundings off where arithmetic in fp32 would be one (2.4e-3 against 1.7e-3 in relative 2-norm); o's
+// probabilities go in as three terms, with fp32's digits, where the table learns (FINE) and for few query rows.  Maxima, sums,
+// statistics and the table's gradient stay in fp32.
 //
 // Times below: us on one MI355X, where a 2 GB copy reaches 5.05 TB/s and an 8192^3 bf16 product of the library 1130 TFLOP/s.  "32 px":
 // 32 samples of a 32x32 map, 4 heads of 64; "64 px": 8 of 64x64, 2 heads of 64, capped scores; "128 px": 4 of 128x128, one head of 64;
@@ -342,16 +344,17 @@ __device__ __forceinline__ int run_first(int n, int runs, int run) { return min(
 // A workgroup owns 128 queries of a head, a wave 32 of them, and streams tiles of keys and values (64 rows, 32 at head size 128) through
 // two LDS buffers: the next tile's loads run under the whole of this one's work.  What bounds it is issue, not a pipe: of the cycles of a
 // SIMD at 128 px the matrix instructions take 34 %, the vector ones (16 exponentials of 4 slots each, 60 others a 32 x 32 block) 54 %, and
-// with two or three waves they overlap little.  Leaving out, one at a time, the exponentials, half of the second product, the bias reads
-// or the tiles' loads shortens it by 9 .. 12 % each; both blocks' first products ahead of the softmax change nothing.  Three workgroups
-// a compute unit at head size 64 (registers and LDS; four spill), two at 128.  32 px 50 without bias, 63 with; 128 px 360 .. 400 (690 ..
-// 760 TFLOP/s; its 512 workgroups are two a compute unit), three times its samples 850 TFLOP/s.  Few workgroups: the keys are cut into
+// with two waves they overlap little (with the cap 32 and 77 %, 64 px).  Leaving out, one at a time, the exponentials, half of the second
+// product, the bias reads or the tiles' loads shortens it by 9 .. 12 % each; both blocks' first products ahead of the softmax change nothing.
+// Three workgroups a compute unit at head size 64 (registers and LDS; four spill), two at 128.  32 px 48 without bias, 59 .. 63 with; 128 px
+// 360 .. 430 (640 .. 760 TFLOP/s; its 512 workgroups are two a compute unit), with a cap of 50 600; three times its samples 780 TFLOP/s, capped
+// 540.  Few workgroups: the keys are cut into
 // `splits` runs, whose fp32 outputs, references and sums a second launch joins.
 // LDS: K[2] V[2] tiles | window | table of the segment's places (BIAS 1).
 // FINE: the probabilities go into the second product as three bf16 terms (24 bits): delta = do . o must be that exact where the fp32
-// gradient of the table is wanted, whose sums cancel.  Its error against 64 bits over forms of 18 to 8192 tokens: one term 5e-4, two
-// 0.6 .. 4e-6, three 0.2 .. 0.7e-6, as fp32 arithmetic leaves.  V's operands serve all three.  32 px: one term 63, two 74, three 84 .. 88
-// (the terms' subtractions, not the products).
+// gradient of the table is wanted, whose sums cancel.  Its error against 64 bits over seven forms of 18 to 4096 tokens: one term 0.5 .. 1.5e-3,
+// two 0.5 .. 2.8e-6, three 0.2 .. 0.6e-6, fp32 torch operations 0.1 .. 1.9e-6.  V's operands serve all three.  32 px: one term 63, two 76, three
+// 84 .. 88 (the terms' subtractions, not the products).
 template <int D, int BIAS, bool CAP, bool FINE>
 __global__ __launch_bounds__(256, D == 128 ? 2 : D == 64 ? 3 : 4) void attn_fwd_kernel(AttnArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -587,8 +590,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a, int D) {
 // however many heads share them, and the keys are cut into `splits` runs for as many workgroups.  Bound by reading keys and values: a
 // wave streams blocks of 32 keys of its own (two buffers, no barrier in the loop), and the waves', then the runs', (maximum, sum,
 // output) are joined in a fixed order.  part: (B, Hkv, splits, 32, D + 2) fp32: output, maximum, sum; one run writes the rows itself.
-// One query, 4 samples of 16384 keys, 8 heads on 2 of 128 (67 MB): 20 + 4, 3.3 TB/s; 256 samples of 1024 keys, 8 heads of 64 (537 MB):
-// 114, 4.7 TB/s.
+// One query, 4 samples of 16384 keys, 8 heads on 2 of 128 (67 MB): 20 + 4 with bias, 3.3 TB/s, 17 + 4 without; 256 samples of 1024 keys, 8 heads
+// of 64 (537 MB): 107, 5.0 TB/s.
 // LDS: for each wave K[2] V[2] of 32 rows; the joining reuses it.
 template <int D> struct WaveDma {
     static constexpr int NP = D / 16;                                // 1 KB pieces of a block
@@ -813,9 +816,11 @@ template <int D> __global__ __launch_bounds__(512) void attn_few_join_kernel(Att
 //   DIAGONALS any other grid: a pair is known by its distance i - j and by whether the column of i wraps (class 0: dx >= 0, class 1:
 //             dx < 0).  ds goes through LDS and a thread adds up one diagonal of the tile; a diagonal stays with its thread (distance
 //             mod 256) over the tiles it crosses and is stored once: part (b, h, query block, class, distance).  Taken where BLOCKS
-//             would do it costs more: 32 px 224 + 18 against 128 + 26, same run.
-// Three products a block where the forward pass has two.  32 px: 68 without bias, 79 with, 107 .. 128 with the table's sums (16 writes and
-// 32 reads of 4 bytes more a lane and block), 64 px 250, line 143 + 9.  Two workgroups a compute unit (three at head size 32).
+//             would do it costs more: 32 px 197 + 22 against 102 + 22.
+// Three products a block where the forward pass has two.  32 px: 67 without bias, 74 .. 79 with, 102 .. 112 with the table's sums (16 writes and
+// 32 reads of 4 bytes more a lane and block; vector instructions 45 %, matrix ones 23 % of a SIMD's cycles), 64 px 229 .. 250, line 138 + 9.  Two
+// workgroups a compute unit; three at head size 32 without the table's sums, with them LDS holds two there as well (and the capped form, kept to
+// the registers of three, spills 84 bytes a lane; at head size 128 28).
 // Few workgroups: the keys are cut into `splits` runs whose fp32 dq a second launch adds up (a run has its own diagonals, and its own blocks).
 // LDS: K[2] V[2] | BLOCKS: a block and its zeros for each wave, DIAGONALS: ds (KT x 128 floats) | window.
 enum { DT_NONE = 0, DT_BLOCKS = 1, DT_DIAGONALS = 2 };
@@ -1169,7 +1174,8 @@ __global__ __launch_bounds__(256) void attn_dist_bucket_kernel(AttnArgs a, const
 // queries x keys, a lane holds one key.  No sum leaves the workgroup; where keys and heads alone are too few workgroups for the chip,
 // the tiles of queries are cut into `splits` runs whose fp32 sums a second launch adds up: part (splits, B, Hkv, Lk, 2 D).
 // Four products a block; the row sums' logarithm and delta come in as the products' initial values, which saves their subtraction.
-// 32 px 82 without bias, 95 .. 107 with, 64 px 239, line 231 + 9.  Two waves a SIMD at head size 64 (three spill), one at 128: dk, dv
+// 32 px 78 without bias, 89 .. 97 with, 64 px 216 .. 247, line 226 .. 239 + 9.  Three waves a SIMD at head size 32 (the capped forms spill 24 .. 32
+// bytes a lane), two at 64 (three spill), one at 128: dk, dv
 // and the wave's own keys and values are 192 registers there, a block's scores and operands the rest of 450; within 256 they spill.
 // LDS: Q[2] dO[2] | lse[2][64] | delta[2][64] | window | table of the segment's places (BIAS 1).
 template <int D, int BIAS, bool CAP>
@@ -1480,9 +1486,10 @@ template <int D> int launch_dkv(const AttnArgs& a, int bias, bool cap, unsigned 
 }
 
 // Few (query, head) pairs over many keys: the number of runs the keys are cut into, 0 for the other form.  Both read a key block once a
-// workgroup, but the other form does it once for every query head and has a workgroup for each, however many keys there are.  us for
-// one query, 4 samples, 8 query heads on 2 of 64, this form / the other: 256 keys 9 / 6, 512 keys 9 / 10, 1024 keys 9 / 17; 64 samples of 512
-// keys 10 / 15; 4 queries, 256 samples of 1024 keys (one run) 26 / 67; 4 samples of 16384 keys, 8 on 2 of 128: 25 / 563.
+// workgroup, but the other form does it once for every query head.  us for one query, 4 samples, 8 query heads on 2 of 64, this form / the other
+// (joins included): 256 keys 6.0 / 7.1, 512 keys 9.6 / 10.1, 1024 keys 9.7 / 13.4; 64 samples of 512 keys 10.4 / 14.5; 4 queries, 256 samples of 1024
+// keys (one run) 27 / 69; 4 samples of 16384 keys, 8 on 2 of 128: 21 / 42.  Where no head shares keys the two are alike (256 samples of 1024 keys, 8 heads
+// of 64: 107 / 104), and up to 256 keys one launch of the other form is within 1 us.
 int few_splits(const rgbd_attn_desc* d) {
     if ((int64_t)d->H / d->Hkv * d->Lq > 32 || d->Lk <= 256 || (int64_t)d->B * d->H * d->Lq >= 1 << 20) return 0;
     const int64_t groups = (int64_t)d->B * d->Hkv, want = d->D == 128 ? 256 : 512;   // workgroups that fit the chip at once (LDS)
@@ -1503,9 +1510,9 @@ template <int D> int launch_few(const AttnArgs& a, bool bias, bool cap, hipStrea
 
 // Runs of query tiles for dk, dv: as many as fill the chip once (one workgroup a compute unit at head size 128, two at 64, three at 32:
 // registers), of at least eight tiles each.  The runs' sums are written and read once more in fp32, which two runs of small heads do
-// not earn back.  us cut / whole, the second launch included: 8 x 1024, 8 query heads on 2 of 64 (4 runs) 50 / 86; 1 x 2048, 4 on 2 of 64
-// (8 runs) 26 / 74; 5 x 713, 6 on 2 of 32 (4 runs) 19 / 33; 2 x 4096, 4 on 2 of 128 (4 runs) 220 / 378; 2 x 2048 x 4 of 128 (2 runs) 67 / 94;
-// but 4 x 2048 x 4 of 64 (2 runs) 52 / 47, 12 x 1024 x 4 of 32 (2 runs) 33 / 26, 4 x 1024 x 4 of 64 in 4 runs of 4 tiles 31 / 25.
+// not earn back.  us cut / whole, the second launch included: 8 x 1024, 8 query heads on 2 of 64 (4 runs) 51 / 90; 1 x 2048, 4 on 2 of 64
+// (8 runs) 25 / 87; 5 x 713, 6 on 2 of 32 (4 runs) 20 / 36; 2 x 4096, 4 on 2 of 128 (4 runs) 222 / 386; 2 x 2048 x 4 of 128 (2 runs) 76 / 102;
+// but 4 x 2048 x 4 of 64 (2 runs) 52 / 49, 12 x 1024 x 4 of 32 (2 runs) 33 / 25, 4 x 1024 x 4 of 64 in 4 runs of 4 tiles 26 / 24.
 int kv_splits(const rgbd_attn_desc* d) {
     const int64_t groups = (int64_t)d->B * d->Hkv * ceil_div(d->Lk, BLK), want = d->D == 128 ? 256 : d->D == 64 ? 512 : 768;
     if (groups == 0) return 1;
@@ -1518,9 +1525,9 @@ int kv_splits(const rgbd_attn_desc* d) {
 
 // Runs of keys for the forward pass and dq where their workgroups leave compute units idle: as many as fill the chip twice over, of at least
 // `least` tiles each (6 forward, 2 for dq); with a workgroup on every compute unit already, only from 32 tiles on.  us cut (with the launch
-// that joins the runs) / whole, forward, dq: 64x64 x 2 heads of 64, one sample (8 runs) 46 / 130, 46 / 148, two samples (4 runs) 55 / 100,
-// 60 / 114; 4 x 32x32 x 4 of 64, capped (2 and 4 runs) 30 / 39, 38 / 46; 5 x 713 x 6 of 32 (2 runs) 30 / 32, 52 / 70; line (2 runs) 144 / 166,
-// 153 / 175; 8 x 16x16 x 4 of 64 (2 runs for dq) 24 / 27; but 8 x 32x32 x 4 of 64, 256 workgroups of 16 tiles, dq 43 / 41.
+// that joins the runs) / whole, forward, dq: 64x64 x 2 heads of 64, one sample (8 runs) 39 / 102, 41 / 118, two samples (4 runs) 55 / 104,
+// 60 / 121; 4 x 32x32 x 4 of 64, capped (2 and 4 runs) 29 / 38, 33 / 45; 5 x 713 x 6 of 32 (2 runs) 29 / 31, 49 / 69; line (2 runs) 145 / 164,
+// 148 / 172; 8 x 16x16 x 4 of 64 (2 runs for dq) 21 / 29; but 8 x 32x32 x 4 of 64, 256 workgroups of 16 tiles, 36 / 33, 42 / 41.
 int key_runs(const rgbd_attn_desc* d, int least) {
     const int64_t groups = (int64_t)d->B * d->H * ceil_div(d->Lq, BLK), tiles = ceil_div(d->Lk, kt_of(d->D));
     if (groups == 0 || (groups >= 256 && tiles < 32)) return 1;

@@ -1718,7 +1718,8 @@ def _vectors(t):
 def group_norm(x, gamma, beta, groups, eps=1e-5, act=None, slope=0.2):
     """act((x - mean) / sqrt(var + eps) * gamma + beta) with mean and variance over each sample's groups of C / groups neighbouring
     channels: x (B, ..., C) bf16 or fp32, channels last, gamma, beta (C,) fp32; act None / "none", "lrelu" (slope) or "silu".  At most
-    65535 samples and 8192 (bf16) or 4096 (fp32) channels, 1024 where C is no multiple of 8 or 4."""
+    65535 samples and 8192 (bf16) or 4096 (fp32) channels, 1024 where C is no multiple of 8 or 4.  The same call repeats bit for bit; a
+    sample's last digits may depend on the batch it is in (sums over many pixels are cut by the number of samples)."""
     x, gamma, beta = _vectors(x), gamma.contiguous(), beta.contiguous()
     if _recorded(x, gamma, beta):
         return _GroupNorm.apply(x, gamma, beta, groups, eps, act, slope)
@@ -1829,7 +1830,11 @@ def attention(q, k, v, table=None, buckets=None, scale=None, cap=0.0, lengths=No
     q_start + i of the grid, key j at token j; values at or below -1e30 (and -inf) leave their offsets out.  A grid of more than one
     row has at most 1024 columns.  -> (B, Lq, H, D) bf16.  Differentiable in q, k, v and table.
 
-    Scores of any size; values within 1e29 (beyond, sums over keys may overflow although their average would not)."""
+    Scores of any size; values within 1e29 (beyond, sums over keys may overflow although their average would not); an infinite or NaN value
+    makes its sample's and head's rows infinite or NaN.  Probabilities are rounded to bf16 for the product with v, but carry 24 bits where the table
+    requires a gradient and for few queries (query heads a key head x Lq at most 32, more than 256 keys): the same call with and without
+    gradients may differ in bf16's last digit.  So may a sample computed in batches of different sizes (sums over keys are cut by the
+    number of samples); the same call repeats bit for bit."""
     spec = (None if scale is None else float(scale), float(cap or 0.0), int(q_start))
     q, k, v = _readable(q), _readable(k), _readable(v)
     table = table.contiguous() if table is not None else None
