@@ -37,10 +37,12 @@ constexpr int WIN_FWD = 20480, WIN_DQ = 10240;
 constexpr float NO_ROW = 0x1p100f;          // log2-sum-exp of a row that is not there: p = exp2(x - 2^100) = 0 for every finite x
 constexpr float NEG_INF = -__builtin_inff();
 // Where a row's sum of probabilities may lie before the forward pass moves its reference.  The output is summed as p v before the division by that
-// sum, so a sum of S takes S from the range of |v| that fp32 can add up: with [2^-10, 2^24], 2^24 being what the largest number of keys reaches
-// next to a reference at their maximum, finite outputs stay finite and keep bf16's digits for |v| in [1e-27, 1e29] (runs of keys joined
-// included), and scores of order 1 over 2^14 keys (a sum near 2^15) never leave it.
-constexpr float SUM_LOW = 0x1p-10f, SUM_HIGH = 0x1p24f;
+// sum, so a sum of S takes S from the range of |v| that fp32 can add up.  Up to 2^24, what the largest number of keys reaches next to a
+// reference at their maximum, finite outputs stay finite for |v| below 1e29 (runs of keys joined included), and scores of order 1 over 2^14
+// keys (a sum near 2^15) never leave it.  Down to 2^-40 the products keep bf16's digits (the matrix unit keeps numbers below 2^-126) for
+// |v| above 1e-27.  A row that has moved pays a subtraction a score, 128 px 385 us against 357: a bias that falls by 50 with the distance puts the
+// first keys of most rows below 2^-40, one that falls by 20 does not (but below 2^-10: 384).
+constexpr float SUM_LOW = 0x1p-40f, SUM_HIGH = 0x1p24f;
 
 struct AttnArgs {
     const unsigned short *q, *k, *v, *d_o, *o, *o_lo;

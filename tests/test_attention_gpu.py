@@ -545,7 +545,8 @@ def test_offsets_beyond_two_to_the_31():
         assert torch.equal(a[n], c[n]), n
 
 
-@pytest.mark.parametrize("far,size", [(35.0, 1e22), (-50.0, 1e-18), (0.0, 1e29), (0.0, 1e-27), (16.0, 1e29), (-6.0, 1e-27)])
+@pytest.mark.parametrize("far,size", [(35.0, 1e22), (-50.0, 1e-18), (0.0, 1e29), (0.0, 1e-27), (16.0, 1e29), (-6.0, 1e-27), (-25.0, 1e-27),
+                                      (-31.0, 1e-27)])
 def test_values_far_from_one(far, size):
     """Scores and values both away from 1: the output is finite and keeps its digits, whatever the sum of the exponentials times a value
     would be.  The whole form, keys in runs, few queries."""
